@@ -1,9 +1,10 @@
 """Builds the two native libraries of the package, in-tree, for sm_100a.
 
 * ``libcie_attention.so`` -- the CUDA kernels and their C ABI
-  (``include/cie_attention.h``, ``include/cie_model_ops.h``), compiled by nvcc
-  from ``csrc/cie_unity.cu`` and ``csrc/model_ops.cu``; the CUDA runtime is
-  linked statically and its symbols are not exported.
+  (``include/cie_attention.h``, ``include/cie_kv_q8.h``,
+  ``include/cie_model_ops.h``), compiled by nvcc from ``csrc/cie_unity.cu``,
+  ``csrc/model_ops.cu`` and ``csrc/sample.cu``; the CUDA runtime is linked
+  statically and its symbols are not exported.
 * ``_cie_torch_ops.so`` -- the ``inference::*`` torch ops
   (``csrc/torch_ops.cpp``) linked against the library above
   (rpath ``$ORIGIN``), built with ``torch.utils.cpp_extension``.
@@ -46,10 +47,10 @@ def _cu_deps():
 
 
 def build_lib(force: bool = False, verbose: bool = False) -> Path:
-    """Two objects linked into one library: the attention kernels
-    (``cie_unity.cu``, --use_fast_math) and the Qwen2 body kernels
+    """Three objects linked into one library: the attention kernels
+    (``cie_unity.cu``, --use_fast_math), the Qwen2 body kernels
     (``model_ops.cu``, IEEE division and library expf / rsqrtf, so that they
-    round like torch's own kernels)."""
+    round like torch's own kernels) and the sampling kernel (``sample.cu``)."""
     if not force and not _stale(LIB, _cu_deps()):
         return LIB
     bdir = PKG / "_build"
@@ -58,7 +59,8 @@ def build_lib(force: bool = False, verbose: bool = False) -> Path:
               "-I", str(INCLUDE), "-I", str(CSRC)]
     if verbose:
         common.insert(1, "-Xptxas=-v")
-    objs = [(CSRC / "cie_unity.cu", ["--use_fast_math"]), (CSRC / "model_ops.cu", [])]
+    objs = [(CSRC / "cie_unity.cu", ["--use_fast_math"]), (CSRC / "model_ops.cu", []),
+            (CSRC / "sample.cu", [])]
     out = []
     for src, extra in objs:
         obj = bdir / (src.stem + ".o")

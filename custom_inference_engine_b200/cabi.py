@@ -217,3 +217,122 @@ def rope_kv_mixed_attention(qkv, cos, sin, k_cache, v_cache, pages, offsets, max
         native.stream_ptr(stream))
     native.check(st, "cie_rope_kv_mixed_attention")
     return out
+
+
+# ---- 8-bit KV pages (include/cie_kv_q8.h) ---------------------------------------
+
+
+def _q8_pool(k_cache, v_cache, kv_scales):
+    return _p(k_cache), _p(v_cache), _p(kv_scales)
+
+
+def _q8_strides(k_cache, n_slots, block_table):
+    return (k_cache.shape[0], n_slots, block_table.stride(0), k_cache.stride(0),
+            k_cache.stride(1))
+
+
+def kv_q8_decode_update(k_cache, v_cache, kv_scales, lens, slot_ids, block_table, k_new, v_new,
+                        stream=None) -> None:
+    """cie_kv_q8_decode_update: int8 pools, fp32 scales (n_pages, 2, H_kv); ``lens``
+    per slot."""
+    st = _entry("cie_kv_q8_decode_update", block_table)(
+        *_q8_pool(k_cache, v_cache, kv_scales), _p(lens), _p(slot_ids), _p(block_table),
+        _p(k_new), _p(v_new), slot_ids.shape[0], k_cache.shape[1], k_cache.shape[3],
+        k_cache.shape[2],
+        *_q8_strides(k_cache, min(lens.shape[0], block_table.shape[0]), block_table),
+        k_new.stride(1), k_new.stride(2), v_new.stride(1), v_new.stride(2),
+        native.stream_ptr(stream))
+    native.check(st, "cie_kv_q8_decode_update")
+
+
+def kv_q8_mixed_update(k_cache, v_cache, kv_scales, cu_seqlens, kv_lens, slot_ids, block_table,
+                       k_new, v_new, stream=None) -> None:
+    """cie_kv_q8_mixed_update: sequence b's rows cu_seqlens[b]..cu_seqlens[b+1] to
+    positions kv_lens[b] onward of its slot."""
+    st = _entry("cie_kv_q8_mixed_update", block_table)(
+        *_q8_pool(k_cache, v_cache, kv_scales), _p(cu_seqlens), _p(kv_lens), _p(slot_ids),
+        _p(block_table), _p(k_new), _p(v_new), slot_ids.shape[0], k_new.shape[1],
+        k_cache.shape[1], k_cache.shape[3], k_cache.shape[2],
+        *_q8_strides(k_cache, block_table.shape[0], block_table), k_new.stride(1),
+        k_new.stride(2), v_new.stride(1), v_new.stride(2), native.stream_ptr(stream))
+    native.check(st, "cie_kv_q8_mixed_update")
+
+
+def rope_kv_q8_decode_update(qkv, cos, sin, k_cache, v_cache, kv_scales, lens, slot_ids,
+                             block_table, out=None, stream=None):
+    """cie_rope_kv_q8_decode_update: rotated q (returned), rotated k and v quantised at
+    each slot's current length."""
+    out, hq = _rope_q_out(qkv, k_cache, out)
+    st = _entry("cie_rope_kv_q8_decode_update", block_table)(
+        _p(qkv), qkv.stride(1), _p(cos), _p(sin), cos.stride(1), _p(out),
+        *_q8_pool(k_cache, v_cache, kv_scales), _p(lens), _p(slot_ids), _p(block_table),
+        slot_ids.shape[0], hq, k_cache.shape[1], k_cache.shape[3], k_cache.shape[2],
+        *_q8_strides(k_cache, min(lens.shape[0], block_table.shape[0]), block_table),
+        native.stream_ptr(stream))
+    native.check(st, "cie_rope_kv_q8_decode_update")
+    return out
+
+
+def rope_kv_q8_mixed_update(qkv, cos, sin, k_cache, v_cache, kv_scales, cu_seqlens, kv_lens,
+                            slot_ids, block_table, out=None, stream=None):
+    """cie_rope_kv_q8_mixed_update: the same for the chunks of a mixed pass."""
+    out, hq = _rope_q_out(qkv, k_cache, out)
+    st = _entry("cie_rope_kv_q8_mixed_update", block_table)(
+        _p(qkv), qkv.stride(1), _p(cos), _p(sin), cos.stride(1), _p(out),
+        *_q8_pool(k_cache, v_cache, kv_scales), _p(cu_seqlens), _p(kv_lens), _p(slot_ids),
+        _p(block_table), slot_ids.shape[0], qkv.shape[1], hq, k_cache.shape[1],
+        k_cache.shape[3], k_cache.shape[2],
+        *_q8_strides(k_cache, block_table.shape[0], block_table), native.stream_ptr(stream))
+    native.check(st, "cie_rope_kv_q8_mixed_update")
+    return out
+
+
+def kv_q8_read(k_cache, v_cache, kv_scales, starts, lens, slot_ids, block_table, k_out, v_out,
+               stream=None) -> None:
+    """cie_kv_q8_read: positions [starts[b], lens[b]) into fp16 pools of the same page
+    ids (``starts`` None: from 0)."""
+    st = _entry("cie_kv_q8_read", block_table)(
+        *_q8_pool(k_cache, v_cache, kv_scales), _p(starts), _p(lens), _p(slot_ids),
+        _p(block_table), _p(k_out), _p(v_out), slot_ids.shape[0], k_cache.shape[1],
+        k_cache.shape[3], k_cache.shape[2],
+        *_q8_strides(k_cache, block_table.shape[0], block_table), k_out.stride(0),
+        k_out.stride(1), native.stream_ptr(stream))
+    native.check(st, "cie_kv_q8_read")
+
+
+def decode_q8_default_splits(batch: int, device: int = 0) -> int:
+    return int(native.lib().cie_decode_q8_default_splits(batch, device))
+
+
+def decode_attention_q8(q, k, v, kv_scales, lens, slot_ids, block_table, out=None,
+                        num_splits: int = 0, workspace: Optional[torch.Tensor] = None,
+                        stream=None) -> torch.Tensor:
+    """cie_decode_attention_q8 on (1, B, H_q, D) q and int8 pools with their scales."""
+    B = slot_ids.shape[0]
+    hq, d = q.shape[2], q.shape[3]
+    S = num_splits if num_splits > 0 else decode_q8_default_splits(B, q.device.index or 0)
+    if out is None:
+        out = torch.empty_like(q)
+    need = decode_workspace_bytes(B, hq, d, S)
+    if need > 0 and workspace is None:
+        workspace = torch.empty(need // 4, dtype=torch.float32, device=q.device)
+    ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    st = _entry("cie_decode_attention_q8", block_table)(
+        _p(q), *_q8_pool(k, v, kv_scales), _p(lens), _p(slot_ids), _p(block_table), _p(out),
+        _p(workspace), ws_bytes, B, hq, k.shape[1], d, k.shape[2],
+        *_q8_strides(k, block_table.shape[0], block_table), S, native.stream_ptr(stream))
+    native.check(st, "cie_decode_attention_q8")
+    return out
+
+
+def sample_rows(logits, uniform, temperature, top_k=None, top_p=None, min_p=None, out=None,
+                stream=None) -> torch.Tensor:
+    """cie_sample_rows: a token per row of (rows, vocab) fp16 logits."""
+    rows, vocab = logits.shape
+    if out is None:
+        out = torch.empty(rows, dtype=torch.int64, device=logits.device)
+    st = native.lib().cie_sample_rows(
+        _p(logits), rows, vocab, logits.stride(0), _p(uniform), _p(temperature), _p(top_k),
+        _p(top_p), _p(min_p), _p(out), native.stream_ptr(stream))
+    native.check(st, "cie_sample_rows")
+    return out

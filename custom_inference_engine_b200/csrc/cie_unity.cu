@@ -5,6 +5,8 @@
 #include "decode_attention.cu"
 #include "decode_noalloc.cu"
 #include "kv_update.cu"
+#include "kv_q8.cu"
+#include "decode_q8.cu"
 #include "lm_head.cu"
 #include "rope_kv.cu"
 #include "mixed_attention.cu"

@@ -16,6 +16,7 @@
 #include <vector>
 
 #include "cie_attention.h"
+#include "cie_kv_q8.h"
 #include "cie_model_ops.h"
 
 namespace {
@@ -401,6 +402,272 @@ at::Tensor rope_kv_decode_attention(const at::Tensor& qkv, const at::Tensor& cos
   return o;
 }
 
+// ---- 8-bit KV pages (cie_kv_q8.h) --------------------------------------------
+
+cie_stream_t current_stream() {
+  return reinterpret_cast<cie_stream_t>(at::cuda::getCurrentCUDAStream().stream());
+}
+
+// Every tensor on the first one's device: a pointer of another device must not
+// reach a kernel. (Messages hold text only: formatting a number into a TORCH_CHECK
+// message ends the process in an extension built against this torch.)
+void check_same_device(const at::Tensor& first, std::initializer_list<at::Tensor> others) {
+  for (const at::Tensor& t : others)
+    TORCH_CHECK(t.device() == first.device(), "all tensors must be on ", first.device().str(),
+                ", got ", t.device().str());
+}
+
+void check_q8_pool(const at::Tensor& k, const at::Tensor& v, const at::Tensor& scales) {
+  TORCH_CHECK(k.is_cuda() && k.scalar_type() == at::kChar && v.scalar_type() == at::kChar,
+              "8-bit caches must be int8 CUDA tensors");
+  TORCH_CHECK(k.dim() == 4 && k.sizes() == v.sizes() && k.strides() == v.strides() &&
+                  k.stride(3) == 1 && k.stride(2) == k.size(3),
+              "k / v must be (n_pages, H_kv, page_size, D) with equal strides and dense rows");
+  TORCH_CHECK(scales.scalar_type() == at::kFloat && scales.is_contiguous() && scales.dim() == 3 &&
+                  scales.size(0) == k.size(0) && scales.size(1) == 2 && scales.size(2) == k.size(1),
+              "kv_scales must be a contiguous float32 (n_pages, 2, H_kv) tensor");
+  check_same_device(k, {v, scales});
+}
+
+void check_q8_tables(const at::Tensor& k, const at::Tensor& slot_ids,
+                     const at::Tensor& block_table) {
+  check_i64(slot_ids, "slot_ids");
+  check_table(block_table);
+  TORCH_CHECK(slot_ids.dim() == 1 && slot_ids.is_contiguous(), "slot_ids must be contiguous (B,)");
+  TORCH_CHECK(block_table.dim() == 2 && block_table.size(1) == k.size(0) &&
+                  block_table.stride(1) == 1,
+              "block_table must be (n_slots, n_pages) with contiguous rows");
+  check_same_device(k, {slot_ids, block_table});
+}
+
+void check_per_sequence(const at::Tensor& t, const at::Tensor& k, int64_t n, const char* name) {
+  check_i64(t, name);
+  TORCH_CHECK(t.dim() == 1 && t.size(0) == n && t.is_contiguous(), name,
+              " must be contiguous 1-D with ", std::to_string(n), " values");
+  check_same_device(k, {t});
+}
+
+void check_q8_rows(const at::Tensor& k, const at::Tensor& k_new, const at::Tensor& v_new) {
+  TORCH_CHECK(k_new.scalar_type() == at::kHalf && v_new.scalar_type() == at::kHalf,
+              "new rows must be float16");
+  TORCH_CHECK(k_new.dim() == 4 && k_new.size(0) == 1 && k_new.size(2) == k.size(1) &&
+                  k_new.size(3) == k.size(3) && k_new.sizes() == v_new.sizes(),
+              "new rows must be (1, T, H_kv, D)");
+  TORCH_CHECK(k_new.stride(3) == 1 && v_new.stride(3) == 1, "new rows need unit inner stride");
+  check_same_device(k, {k_new, v_new});
+}
+
+void check_q8_rope(const at::Tensor& qkv, const at::Tensor& cos, const at::Tensor& sin,
+                   const at::Tensor& k) {
+  TORCH_CHECK(qkv.scalar_type() == at::kHalf && cos.scalar_type() == at::kHalf &&
+                  sin.scalar_type() == at::kHalf,
+              "qkv / cos / sin must be float16");
+  TORCH_CHECK(qkv.dim() == 3 && qkv.size(0) == 1 && qkv.stride(2) == 1,
+              "qkv must be (1, T, (H_q + 2 H_kv) * D) with unit inner stride");
+  TORCH_CHECK(k.size(3) > 0 && qkv.size(2) % k.size(3) == 0 &&
+                  qkv.size(2) / k.size(3) > 2 * k.size(1),
+              "qkv width must be (H_q + 2 H_kv) * D");
+  TORCH_CHECK(cos.dim() == 3 && cos.sizes() == sin.sizes() && cos.strides() == sin.strides() &&
+                  cos.size(0) == 1 && cos.size(1) == qkv.size(1) && cos.size(2) == k.size(3) &&
+                  cos.stride(2) == 1,
+              "cos / sin must be (1, T, D) with unit inner stride");
+  check_same_device(k, {qkv, cos, sin});
+}
+
+// Slots that both the lengths (per slot) and the block table have.
+int64_t slots_of(const at::Tensor& lens, const at::Tensor& block_table) {
+  return std::min(lens.size(0), block_table.size(0));
+}
+
+void check_slot_lens(const at::Tensor& lens, const at::Tensor& k) {
+  check_i64(lens, "lens");
+  TORCH_CHECK(lens.dim() == 1 && lens.is_contiguous(), "lens (per slot) must be contiguous 1-D");
+  check_same_device(k, {lens});
+}
+
+void kv_q8_decode_update(at::Tensor& k_cache, at::Tensor& v_cache, at::Tensor& kv_scales,
+                         const at::Tensor& lens, const at::Tensor& slot_ids,
+                         const at::Tensor& block_table, const at::Tensor& k_new,
+                         const at::Tensor& v_new) {
+  check_q8_pool(k_cache, v_cache, kv_scales);
+  check_q8_tables(k_cache, slot_ids, block_table);
+  check_slot_lens(lens, k_cache);
+  check_q8_rows(k_cache, k_new, v_new);
+  TORCH_CHECK(k_new.size(1) == slot_ids.size(0), "one new row per slot id");
+  c10::cuda::CUDAGuard guard(k_cache.device());
+  const int st = with_table(
+      block_table,
+      [&](auto fn, auto* table) {
+        return fn(k_cache.data_ptr(), v_cache.data_ptr(), kv_scales.data_ptr<float>(),
+                  lens.data_ptr<int64_t>(), slot_ids.data_ptr<int64_t>(), table,
+                  k_new.data_ptr(), v_new.data_ptr(), static_cast<int>(slot_ids.size(0)),
+                  static_cast<int>(k_cache.size(1)), static_cast<int>(k_cache.size(3)),
+                  static_cast<int>(k_cache.size(2)), k_cache.size(0), slots_of(lens, block_table),
+                  block_table.stride(0), k_cache.stride(0), k_cache.stride(1), k_new.stride(1),
+                  k_new.stride(2), v_new.stride(1), v_new.stride(2), current_stream());
+      },
+      cie_kv_q8_decode_update, cie_kv_q8_decode_update_bt32);
+  check_status(st, "kv_q8_decode_update");
+}
+
+void kv_q8_mixed_update(at::Tensor& k_cache, at::Tensor& v_cache, at::Tensor& kv_scales,
+                        const at::Tensor& cu_seqlens, const at::Tensor& kv_lens,
+                        const at::Tensor& slot_ids, const at::Tensor& block_table,
+                        const at::Tensor& k_new, const at::Tensor& v_new) {
+  check_q8_pool(k_cache, v_cache, kv_scales);
+  check_q8_tables(k_cache, slot_ids, block_table);
+  const int64_t B = slot_ids.size(0);
+  check_per_sequence(cu_seqlens, k_cache, B + 1, "cu_seqlens");
+  check_per_sequence(kv_lens, k_cache, B, "kv_lens");
+  check_q8_rows(k_cache, k_new, v_new);
+  c10::cuda::CUDAGuard guard(k_cache.device());
+  const int st = with_table(
+      block_table,
+      [&](auto fn, auto* table) {
+        return fn(k_cache.data_ptr(), v_cache.data_ptr(), kv_scales.data_ptr<float>(),
+                  cu_seqlens.data_ptr<int64_t>(), kv_lens.data_ptr<int64_t>(),
+                  slot_ids.data_ptr<int64_t>(), table, k_new.data_ptr(), v_new.data_ptr(),
+                  static_cast<int>(B), k_new.size(1), static_cast<int>(k_cache.size(1)),
+                  static_cast<int>(k_cache.size(3)), static_cast<int>(k_cache.size(2)),
+                  k_cache.size(0), block_table.size(0), block_table.stride(0), k_cache.stride(0),
+                  k_cache.stride(1), k_new.stride(1), k_new.stride(2), v_new.stride(1),
+                  v_new.stride(2), current_stream());
+      },
+      cie_kv_q8_mixed_update, cie_kv_q8_mixed_update_bt32);
+  check_status(st, "kv_q8_mixed_update");
+}
+
+at::Tensor rope_kv_q8_decode_update(const at::Tensor& qkv, const at::Tensor& cos,
+                                    const at::Tensor& sin, at::Tensor& k_cache,
+                                    at::Tensor& v_cache, at::Tensor& kv_scales,
+                                    const at::Tensor& lens, const at::Tensor& slot_ids,
+                                    const at::Tensor& block_table) {
+  check_q8_pool(k_cache, v_cache, kv_scales);
+  check_q8_rope(qkv, cos, sin, k_cache);
+  check_q8_tables(k_cache, slot_ids, block_table);
+  check_slot_lens(lens, k_cache);
+  TORCH_CHECK(slot_ids.size(0) == qkv.size(1), "one token per slot id");
+  c10::cuda::CUDAGuard guard(qkv.device());
+  at::Tensor q = rope_out(qkv, k_cache);
+  const int st = with_table(
+      block_table,
+      [&](auto fn, auto* table) {
+        return fn(qkv.data_ptr(), qkv.stride(1), cos.data_ptr(), sin.data_ptr(), cos.stride(1),
+                  q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                  kv_scales.data_ptr<float>(), lens.data_ptr<int64_t>(),
+                  slot_ids.data_ptr<int64_t>(), table, static_cast<int>(slot_ids.size(0)),
+                  static_cast<int>(q.size(2)), static_cast<int>(k_cache.size(1)),
+                  static_cast<int>(k_cache.size(3)), static_cast<int>(k_cache.size(2)),
+                  k_cache.size(0), slots_of(lens, block_table), block_table.stride(0),
+                  k_cache.stride(0), k_cache.stride(1), current_stream());
+      },
+      cie_rope_kv_q8_decode_update, cie_rope_kv_q8_decode_update_bt32);
+  check_status(st, "rope_kv_q8_decode_update");
+  return q;
+}
+
+at::Tensor rope_kv_q8_mixed_update(const at::Tensor& qkv, const at::Tensor& cos,
+                                   const at::Tensor& sin, at::Tensor& k_cache,
+                                   at::Tensor& v_cache, at::Tensor& kv_scales,
+                                   const at::Tensor& cu_seqlens, const at::Tensor& kv_lens,
+                                   const at::Tensor& slot_ids, const at::Tensor& block_table) {
+  check_q8_pool(k_cache, v_cache, kv_scales);
+  check_q8_rope(qkv, cos, sin, k_cache);
+  check_q8_tables(k_cache, slot_ids, block_table);
+  const int64_t B = slot_ids.size(0);
+  check_per_sequence(cu_seqlens, k_cache, B + 1, "cu_seqlens");
+  check_per_sequence(kv_lens, k_cache, B, "kv_lens");
+  c10::cuda::CUDAGuard guard(qkv.device());
+  at::Tensor q = rope_out(qkv, k_cache);
+  const int st = with_table(
+      block_table,
+      [&](auto fn, auto* table) {
+        return fn(qkv.data_ptr(), qkv.stride(1), cos.data_ptr(), sin.data_ptr(), cos.stride(1),
+                  q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                  kv_scales.data_ptr<float>(), cu_seqlens.data_ptr<int64_t>(),
+                  kv_lens.data_ptr<int64_t>(), slot_ids.data_ptr<int64_t>(), table,
+                  static_cast<int>(B), qkv.size(1), static_cast<int>(q.size(2)),
+                  static_cast<int>(k_cache.size(1)), static_cast<int>(k_cache.size(3)),
+                  static_cast<int>(k_cache.size(2)), k_cache.size(0), block_table.size(0),
+                  block_table.stride(0), k_cache.stride(0), k_cache.stride(1), current_stream());
+      },
+      cie_rope_kv_q8_mixed_update, cie_rope_kv_q8_mixed_update_bt32);
+  check_status(st, "rope_kv_q8_mixed_update");
+  return q;
+}
+
+void kv_q8_read(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& kv_scales,
+                const std::optional<at::Tensor>& starts, const at::Tensor& lens,
+                const at::Tensor& slot_ids, const at::Tensor& block_table, at::Tensor& k_out,
+                at::Tensor& v_out) {
+  check_q8_pool(k_cache, v_cache, kv_scales);
+  check_q8_tables(k_cache, slot_ids, block_table);
+  const int64_t B = slot_ids.size(0);
+  check_per_sequence(lens, k_cache, B, "lens");
+  if (starts) check_per_sequence(*starts, k_cache, B, "starts");
+  TORCH_CHECK(k_out.scalar_type() == at::kHalf && v_out.scalar_type() == at::kHalf,
+              "k_out / v_out must be float16");
+  TORCH_CHECK(k_out.sizes() == k_cache.sizes() && k_out.sizes() == v_out.sizes() &&
+                  k_out.strides() == v_out.strides() && k_out.stride(3) == 1 &&
+                  k_out.stride(2) == k_out.size(3),
+              "k_out / v_out must have the cache's shape, equal strides and dense rows");
+  check_same_device(k_cache, {k_out, v_out});
+  c10::cuda::CUDAGuard guard(k_cache.device());
+  const int st = with_table(
+      block_table,
+      [&](auto fn, auto* table) {
+        return fn(k_cache.data_ptr(), v_cache.data_ptr(), kv_scales.data_ptr<float>(),
+                  starts ? starts->data_ptr<int64_t>() : nullptr, lens.data_ptr<int64_t>(),
+                  slot_ids.data_ptr<int64_t>(), table, k_out.data_ptr(), v_out.data_ptr(),
+                  static_cast<int>(B), static_cast<int>(k_cache.size(1)),
+                  static_cast<int>(k_cache.size(3)), static_cast<int>(k_cache.size(2)),
+                  k_cache.size(0), block_table.size(0), block_table.stride(0), k_cache.stride(0),
+                  k_cache.stride(1), k_out.stride(0), k_out.stride(1), current_stream());
+      },
+      cie_kv_q8_read, cie_kv_q8_read_bt32);
+  check_status(st, "kv_q8_read");
+}
+
+at::Tensor gqa_decode_attention_q8(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                   const at::Tensor& kv_scales, const at::Tensor& lens,
+                                   const at::Tensor& slot_ids, const at::Tensor& block_table) {
+  check_q8_pool(k, v, kv_scales);
+  check_q8_tables(k, slot_ids, block_table);
+  const int64_t B = slot_ids.size(0);
+  check_per_sequence(lens, k, B, "lens");
+  TORCH_CHECK(q.scalar_type() == at::kHalf && q.dim() == 4 && q.size(0) == 1 && q.size(1) == B &&
+                  q.is_contiguous(),
+              "q must be a contiguous float16 (1, B, H_q, D) tensor");
+  TORCH_CHECK(k.size(1) > 0 && q.size(2) % k.size(1) == 0 && q.size(3) == k.size(3),
+              "H_q must be a multiple of H_kv and head_dim the cache's");
+  check_same_device(k, {q});
+  c10::cuda::CUDAGuard guard(q.device());
+  at::Tensor o = at::empty_like(q);
+  if (B == 0) return o;
+  const int S = cie_decode_q8_default_splits(static_cast<int>(B), q.get_device());
+  const size_t ws_bytes =
+      cie_decode_workspace_bytes(static_cast<int>(B), static_cast<int>(q.size(2)),
+                                 static_cast<int>(q.size(3)), S);
+  at::Tensor ws;
+  if (ws_bytes > 0)
+    ws = at::empty({static_cast<int64_t>(ws_bytes / sizeof(float))},
+                   q.options().dtype(at::kFloat));
+  const int st = with_table(
+      block_table,
+      [&](auto fn, auto* table) {
+        return fn(q.data_ptr(), k.data_ptr(), v.data_ptr(), kv_scales.data_ptr<float>(),
+                  lens.data_ptr<int64_t>(), slot_ids.data_ptr<int64_t>(), table, o.data_ptr(),
+                  ws_bytes > 0 ? ws.data_ptr() : nullptr, ws_bytes, static_cast<int>(B),
+                  static_cast<int>(q.size(2)), static_cast<int>(k.size(1)),
+                  static_cast<int>(q.size(3)), static_cast<int>(k.size(2)), k.size(0),
+                  block_table.size(0), block_table.stride(0), k.stride(0), k.stride(1), S,
+                  current_stream());
+      },
+      cie_decode_attention_q8, cie_decode_attention_q8_bt32);
+  check_status(st, "gqa_decode_attention_q8");
+  return o;
+}
+
 // ---- Qwen2 body helpers (cie_model_ops.h) ----------------------------------
 
 void check_rows(const at::Tensor& t, const char* name) {
@@ -507,6 +774,35 @@ at::Tensor lm_head_argmax(const at::Tensor& hidden, const at::Tensor& weight) {
   return out;
 }
 
+// A token per row of logits (..., vocab) from given random numbers (cie_sample_rows).
+at::Tensor sample_rows(const at::Tensor& logits, const at::Tensor& uniform,
+                       const at::Tensor& temperature, const std::optional<at::Tensor>& top_k,
+                       const std::optional<at::Tensor>& top_p,
+                       const std::optional<at::Tensor>& min_p) {
+  check_rows(logits, "logits");
+  const int64_t rows = logits.numel() / std::max<int64_t>(logits.size(-1), 1);
+  auto per_row = [&](const at::Tensor& t, at::ScalarType type, const char* name) {
+    TORCH_CHECK(t.scalar_type() == type && t.is_contiguous() && t.numel() == rows, name,
+                " must be a contiguous ", c10::toString(type), " tensor with one value per row");
+    check_same_device(logits, {t});
+  };
+  per_row(uniform, at::kFloat, "uniform");
+  per_row(temperature, at::kFloat, "temperature");
+  if (top_k) per_row(*top_k, at::kLong, "top_k");
+  if (top_p) per_row(*top_p, at::kFloat, "top_p");
+  if (min_p) per_row(*min_p, at::kFloat, "min_p");
+  c10::cuda::CUDAGuard guard(logits.device());
+  std::vector<int64_t> shape(logits.sizes().begin(), logits.sizes().end() - 1);
+  at::Tensor out = at::empty(shape, logits.options().dtype(at::kLong));
+  const int st = cie_sample_rows(
+      logits.data_ptr(), rows, logits.size(-1), row_stride(logits), uniform.data_ptr<float>(),
+      temperature.data_ptr<float>(), top_k ? top_k->data_ptr<int64_t>() : nullptr,
+      top_p ? top_p->data_ptr<float>() : nullptr, min_p ? min_p->data_ptr<float>() : nullptr,
+      out.data_ptr<int64_t>(), current_stream());
+  check_status(st, "sample_rows");
+  return out;
+}
+
 }  // namespace
 
 TORCH_LIBRARY(inference, m) {
@@ -538,11 +834,35 @@ TORCH_LIBRARY(inference, m) {
   m.def(
       "rope_kv_decode_attention(Tensor qkv, Tensor cos, Tensor sin, Tensor(a!) k_cache, "
       "Tensor(b!) v_cache, Tensor lens, Tensor slot_ids, Tensor block_table) -> Tensor");
+  m.def(
+      "kv_q8_decode_update(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!) kv_scales, "
+      "Tensor lens, Tensor slot_ids, Tensor block_table, Tensor k_new, Tensor v_new) -> ()");
+  m.def(
+      "kv_q8_mixed_update(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!) kv_scales, "
+      "Tensor cu_seqlens, Tensor kv_lens, Tensor slot_ids, Tensor block_table, Tensor k_new, "
+      "Tensor v_new) -> ()");
+  m.def(
+      "rope_kv_q8_decode_update(Tensor qkv, Tensor cos, Tensor sin, Tensor(a!) k_cache, "
+      "Tensor(b!) v_cache, Tensor(c!) kv_scales, Tensor lens, Tensor slot_ids, "
+      "Tensor block_table) -> Tensor");
+  m.def(
+      "rope_kv_q8_mixed_update(Tensor qkv, Tensor cos, Tensor sin, Tensor(a!) k_cache, "
+      "Tensor(b!) v_cache, Tensor(c!) kv_scales, Tensor cu_seqlens, Tensor kv_lens, "
+      "Tensor slot_ids, Tensor block_table) -> Tensor");
+  m.def(
+      "kv_q8_read(Tensor k_cache, Tensor v_cache, Tensor kv_scales, Tensor? starts, Tensor lens, "
+      "Tensor slot_ids, Tensor block_table, Tensor(a!) k_out, Tensor(b!) v_out) -> ()");
+  m.def(
+      "gqa_decode_attention_q8(Tensor q, Tensor k, Tensor v, Tensor kv_scales, Tensor lens, "
+      "Tensor slot_ids, Tensor block_table) -> Tensor");
   m.def("rms_norm(Tensor x, Tensor weight, float eps) -> Tensor");
   m.def("add_rms_norm(Tensor(a!) residual, Tensor delta, Tensor weight, float eps) -> Tensor");
   m.def("silu_and_mul(Tensor gate_up) -> Tensor");
   m.def("argmax_rows(Tensor x) -> Tensor");
   m.def("lm_head_argmax(Tensor hidden, Tensor weight) -> Tensor");
+  m.def(
+      "sample_rows(Tensor logits, Tensor uniform, Tensor temperature, Tensor? top_k=None, "
+      "Tensor? top_p=None, Tensor? min_p=None) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(inference, CUDA, m) {
@@ -560,4 +880,11 @@ TORCH_LIBRARY_IMPL(inference, CUDA, m) {
   m.impl("silu_and_mul", &silu_and_mul);
   m.impl("argmax_rows", &argmax_rows);
   m.impl("lm_head_argmax", &lm_head_argmax);
+  m.impl("kv_q8_decode_update", &kv_q8_decode_update);
+  m.impl("kv_q8_mixed_update", &kv_q8_mixed_update);
+  m.impl("rope_kv_q8_decode_update", &rope_kv_q8_decode_update);
+  m.impl("rope_kv_q8_mixed_update", &rope_kv_q8_mixed_update);
+  m.impl("kv_q8_read", &kv_q8_read);
+  m.impl("gqa_decode_attention_q8", &gqa_decode_attention_q8);
+  m.impl("sample_rows", &sample_rows);
 }

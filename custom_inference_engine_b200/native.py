@@ -29,7 +29,7 @@ c_int = ctypes.c_int
 c_ptr = ctypes.c_void_p
 c_size = ctypes.c_size_t
 
-# name -> (restype, argtypes); mirrors include/cie_attention.h and include/cie_model_ops.h
+# name -> (restype, argtypes); mirrors the headers in include/
 SIGNATURES = {
     "cie_version": (c_int, []),
     "cie_status_string": (ctypes.c_char_p, [c_int]),
@@ -70,10 +70,26 @@ SIGNATURES = {
                                             c_int, c_int, c_i64, c_i64, c_i64, c_i64, c_i64,
                                             c_int, c_ptr]),
 }
+SIGNATURES.update({
+    # include/cie_kv_q8.h
+    "cie_kv_q8_decode_update": (c_int, [c_ptr] * 8 + [c_int] * 4 + [c_i64] * 9 + [c_ptr]),
+    "cie_kv_q8_mixed_update": (c_int, [c_ptr] * 9 + [c_int, c_i64] + [c_int] * 3 + [c_i64] * 9
+                               + [c_ptr]),
+    "cie_rope_kv_q8_decode_update": (c_int, [c_ptr, c_i64, c_ptr, c_ptr, c_i64] + [c_ptr] * 7
+                                     + [c_int] * 5 + [c_i64] * 5 + [c_ptr]),
+    "cie_rope_kv_q8_mixed_update": (c_int, [c_ptr, c_i64, c_ptr, c_ptr, c_i64] + [c_ptr] * 8
+                                    + [c_int, c_i64] + [c_int] * 4 + [c_i64] * 5 + [c_ptr]),
+    "cie_kv_q8_read": (c_int, [c_ptr] * 9 + [c_int] * 4 + [c_i64] * 7 + [c_ptr]),
+    "cie_decode_q8_default_splits": (c_int, [c_int, c_int]),
+    "cie_decode_attention_q8": (c_int, [c_ptr] * 9 + [c_size] + [c_int] * 5 + [c_i64] * 5
+                                + [c_int, c_ptr]),
+})
 # the int32-block-table variants take the same arguments
 for _name in ("cie_decode_attention", "cie_mixed_attention", "cie_kv_decode_update",
               "cie_rope_kv_decode_update", "cie_rope_kv_decode_attention",
-              "cie_rope_kv_mixed_attention"):
+              "cie_rope_kv_mixed_attention", "cie_kv_q8_decode_update", "cie_kv_q8_mixed_update",
+              "cie_rope_kv_q8_decode_update", "cie_rope_kv_q8_mixed_update", "cie_kv_q8_read",
+              "cie_decode_attention_q8"):
     SIGNATURES[_name + "_bt32"] = SIGNATURES[_name]
 SIGNATURES.update({
     # include/cie_model_ops.h
@@ -85,6 +101,7 @@ SIGNATURES.update({
     "cie_lm_head_argmax_workspace_bytes": (c_size, [c_int, c_i64, c_int]),
     "cie_lm_head_argmax": (c_int, [c_ptr, c_i64, c_ptr, c_i64, c_int, c_int, c_i64, c_ptr,
                                    c_i64, c_ptr, c_ptr, c_size, c_ptr]),
+    "cie_sample_rows": (c_int, [c_ptr, c_i64, c_i64, c_i64] + [c_ptr] * 7),
 })
 
 CIE_OK = 0
@@ -207,6 +224,38 @@ def _register_fakes() -> None:
     @torch.library.register_fake("inference::lm_head_argmax")
     def _lm_head_argmax_fake(hidden, weight):
         return hidden.new_empty(hidden.shape[:-1], dtype=torch.long)
+
+    @torch.library.register_fake("inference::sample_rows")
+    def _sample_fake(logits, uniform, temperature, top_k=None, top_p=None, min_p=None):
+        return logits.new_empty(logits.shape[:-1], dtype=torch.long)
+
+    @torch.library.register_fake("inference::kv_q8_decode_update")
+    def _q8_dec_fake(k_cache, v_cache, kv_scales, lens, slot_ids, block_table, k_new, v_new):
+        return None
+
+    @torch.library.register_fake("inference::kv_q8_mixed_update")
+    def _q8_mix_fake(k_cache, v_cache, kv_scales, cu_seqlens, kv_lens, slot_ids, block_table,
+                     k_new, v_new):
+        return None
+
+    @torch.library.register_fake("inference::rope_kv_q8_decode_update")
+    def _rope_q8_dec_fake(qkv, cos, sin, k_cache, v_cache, kv_scales, lens, slot_ids,
+                          block_table):
+        return _rope_out(qkv, k_cache)
+
+    @torch.library.register_fake("inference::rope_kv_q8_mixed_update")
+    def _rope_q8_mix_fake(qkv, cos, sin, k_cache, v_cache, kv_scales, cu_seqlens, kv_lens,
+                          slot_ids, block_table):
+        return _rope_out(qkv, k_cache)
+
+    @torch.library.register_fake("inference::kv_q8_read")
+    def _q8_read_fake(k_cache, v_cache, kv_scales, starts, lens, slot_ids, block_table, k_out,
+                      v_out):
+        return None
+
+    @torch.library.register_fake("inference::gqa_decode_attention_q8")
+    def _decode_q8_fake(q, k, v, kv_scales, lens, slot_ids, block_table):
+        return torch.empty_like(q)
 
     @torch.library.register_fake("inference::silu_and_mul")
     def _silu_mul_fake(gate_up):

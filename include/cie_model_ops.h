@@ -81,6 +81,29 @@ int cie_lm_head_argmax(const void* hidden, int64_t hidden_stride, const void* we
                        void* logits, int64_t logits_stride, int64_t* tokens, void* workspace,
                        size_t workspace_bytes, cie_stream_t stream);
 
+/*
+ * A sampled token per row of fp16 logits, from a given random number: the row's
+ * tokens sorted by logit (descending; equal logits: lowest index first) have the
+ * weights w = exp((logit - max) / temperature[r]); the kept tokens are the
+ * shortest of three prefixes of that order --
+ *   top_k[r]  the first top_k tokens (<= 0 or >= vocab: all),
+ *   top_p[r]  the shortest prefix whose mass is >= top_p times the mass of the
+ *             top_k prefix (>= 1: all),
+ *   min_p[r]  the tokens with w >= min_p (the maximum's w is 1; <= 0: all) --
+ * and never fewer than one; out[r] is the first token of the order at which the
+ * cumulative mass exceeds uniform[r] * (mass of the kept tokens), uniform in
+ * [0, 1) (a number outside gives the first or the last kept token). Weights
+ * and masses are fp64. temperature[r] <= 0 or NaN gives the row's first
+ * maximum, cie_argmax_rows' token, and so does a row that holds a NaN (its
+ * first NaN). Tokens at -inf have no weight; a row of nothing else gives token
+ * 0; +inf logits share all of the mass. -0 and +0 are equal. top_k (int64),
+ * top_p and min_p (fp32) may be NULL (off). Rows `stride` elements apart
+ * (16-byte aligned rows are read 8 values at a time). vocab <= 524224; out int64.
+ */
+int cie_sample_rows(const void* logits, int64_t rows, int64_t vocab, int64_t stride,
+                    const float* uniform, const float* temperature, const int64_t* top_k,
+                    const float* top_p, const float* min_p, int64_t* out, cie_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
