@@ -32,12 +32,14 @@ namespace sample {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 512;
 constexpr int kKeys = 1 << 16;
 constexpr int kChunks = 256;              // of 256 keys, 8 per lane
 constexpr int kMaxPart = 65528;           // tokens of a part: multiple of 8 below 2^16
 constexpr int kMaxCluster = 8;
-constexpr unsigned int kMinusInf = 0xFC00;  // key of -inf; key 0 is NaN, 0x3FF +inf
+// keys of some values
+constexpr unsigned int kPlusInf = 0x3FF, kFirstFinite = 0x400, kPlusZero = 0x7FFF;
+constexpr unsigned int kMinusZero = 0x8000, kMinusInf = 0xFC00;
 
 struct Params {
   const __half* logits;
@@ -50,70 +52,132 @@ struct Params {
   int64_t* out;
   int vocab;
   int part;                 // tokens per CTA, multiple of 8
-  int vec;                  // rows start on 16-byte boundaries
 };
 
-struct Shared {
+struct alignas(16) Shared {
   uint32_t hist[kKeys / 2];       // counter of key d: half d & 1 of word d >> 1
-  double mass[kChunks];           // CTA 0: per chunk
-  int count[kChunks];
-  int above[kChunks];             // tokens with w >= min_p
+  // CTA 0, per chunk: mass and tokens, those of all chunks before, and those that min-p
+  // keeps (`some` says that it drops any)
+  double mass[kChunks], mass_before[kChunks], mass_above[kChunks];
+  int count[kChunks], before[kChunks], above[kChunks];
+  int some;
   int warp_sum[kThreads / 32];
-  unsigned int top;               // smallest key (largest logit) of this CTA's part
-  unsigned int key;               // the sampled token's key and its rank among the
-  int rank;                       // row's tokens of that key
+  unsigned int top, bottom;       // smallest and largest key of this CTA's part
+  unsigned int tops[kMaxCluster], bottoms[kMaxCluster];  // and of every part
+  unsigned int key;               // the sampled token's key and its rank among this
+  int rank;                       // part's tokens of that key (negative: not here)
 };
 
-// Ordered key of a fp16 value: 0 for NaN, then descending values; -0 and +0 share one.
+// Ordered keys of two fp16 values: descending values ascend, NaNs lie below +inf's key
+// and above -inf's, -0 (0x8000) comes after +0 (0x7fff).
+__device__ __forceinline__ uint32_t keys_of2(uint32_t bits) {
+  return bits ^ ((~bits >> 15 & 0x00010001u) * 0x7fffu);  // 0x7fff - b for positive b
+}
+
+// The key under which a token is looked up: one for -0 and +0, one (0) for every NaN.
 __device__ __forceinline__ unsigned int key_of(unsigned int bits) {
   if ((bits & 0x7fffu) > 0x7c00u) return 0u;
   if (bits == 0x8000u) bits = 0u;
   return (bits & 0x8000u) ? bits : 0x7fffu - bits;
 }
 
-__device__ __forceinline__ double value_of(unsigned int key) {
+// 2^e for -1022 <= e <= 1023.
+__device__ __forceinline__ double exp2_of(int e) { return __hiloint2double((1023 + e) << 20, 0); }
+
+// The number of tokens c (below 2^32) as a double.
+__device__ __forceinline__ double as_double(unsigned int c) {
+  return __hiloint2double(0x43300000, static_cast<int>(c)) - 4503599627370496.0;
+}
+
+// fp16 value of a finite key, and the step (< 0) to the next key's value in its binade
+// of 1024 keys.
+__device__ __forceinline__ double value_of(unsigned int key, double& step) {
   const unsigned int bits = key >= 0x8000u ? key : 0x7fffu - key;
-  return static_cast<double>(__half2float(__ushort_as_half(static_cast<unsigned short>(bits))));
+  const int binade = static_cast<int>(bits >> 10 & 31u);
+  const unsigned int whole = (bits & 1023u) + (binade ? 1024u : 0u);
+  const double ulp = exp2_of(max(binade, 1) - 25);
+  step = -ulp;
+  return as_double(whole) * ((bits & 0x8000u) ? -ulp : ulp);
 }
 
-__device__ __forceinline__ double weight(unsigned int key, unsigned int top, double peak,
-                                         double temp) {
-  if (key == top) return 1.0;
-  if (key >= kMinusInf) return 0.0;
-  return exp((value_of(key) - peak) / temp);
+// exp(x) for -700 <= x <= 0, without a branch, so that several run interleaved: x =
+// k ln 2 + r with |r| <= ln 2 / 2 (ln 2 in two parts, after Cody and Waite), 2^k in the
+// exponent and the Taylor series of exp(r) through r^13, whose remainder is below 2^-57.
+__device__ __forceinline__ double exp_above_700(double x) {
+  constexpr double kShift = 6755399441055744.0;  // 1.5 * 2^52: the sum's low word is k
+  const double t = fma(x, 1.4426950408889634, kShift), k = t - kShift;
+  const double r = fma(k, -2.3190468138462996e-17, fma(k, -0.6931471805599453, x));
+  const double r2 = r * r, r4 = r2 * r2;
+  const double a = fma(r2, fma(r, 1.0 / 6, 0.5), fma(r, 1.0, 1.0));
+  const double b = fma(r2, fma(r, 1.0 / 5040, 1.0 / 720), fma(r, 1.0 / 120, 1.0 / 24));
+  const double c = fma(r2, fma(r, 1.0 / 39916800, 1.0 / 3628800), fma(r, 1.0 / 362880, 1.0 / 40320));
+  const double d = fma(r, 1.0 / 6227020800, 1.0 / 479001600);
+  const double p = fma(r4, fma(r4, fma(r4, d, c), b), a);
+  return __hiloint2double(__double2hiint(p) + (__double2loint(t) << 20), __double2loint(p));
 }
 
-// Counters of keys [8 j, 8 j + 8) summed over the cluster.
-__device__ __forceinline__ void counts8(cg::cluster_group& cluster, Shared* sh, int parts, int j,
-                                        int (&c)[8]) {
+// The weights of neighbouring keys of one binade: key first + e weighs
+// base * ratio^(e - shift) from e = shift on and nothing before, where shift > 0 only
+// if first lies above the row's largest logit. Two exponentials for 8 or 32 weights,
+// each within 2^-47 of exp((value - peak) / temp).
+struct Weights {
+  double base;
+  int shift;
+  bool tiny;  // some of the keys may weigh 0: take base from Scale::exact
+};
+
+struct Scale {
+  unsigned int top;      // the row's smallest key
+  double peak, inv_temp; // its value, 1 / temperature
+
+  // the weights of two neighbouring keys of first's binade, one by the other
+  __device__ __forceinline__ double ratio(unsigned int first) const {
+    double step;
+    value_of(first, step);
+    const double x = step * inv_temp;
+    return top < kFirstFinite || first >= kMinusInf || x < -700.0 ? 0.0 : exp_above_700(fmax(x, -700.0));
+  }
+
+  __device__ __forceinline__ Weights from(unsigned int first, double keys = 8.0) const {
+    const unsigned int at = max(first, top);
+    double step;
+    const double x = (value_of(at, step) - peak) * inv_temp;
+    // all of the weight is the largest logit's when that is +inf; -inf has none
+    const bool tiny = !(fma(keys * step, inv_temp, x) > -700.0) || top < kFirstFinite ||
+                      first >= kMinusInf;
+    return Weights{exp_above_700(tiny ? -700.0 : x), static_cast<int>(at - first), tiny};
+  }
+
+  __device__ __forceinline__ double exact(unsigned int first) const {
+    const unsigned int at = max(first, top);
+    if (at == top) return 1.0;
+    if (top < kFirstFinite || first >= kMinusInf) return 0.0;
+    double step;
+    return exp((value_of(at, step) - peak) * inv_temp);
+  }
+};
+
+// Counters of keys [8 j, 8 j + 8) summed over the cluster, from part `first` on (each
+// part begins with its own, so that no part is read by all at once).
+template <int kParts>
+__device__ __forceinline__ void counts8(cg::cluster_group& cluster, Shared* sh, int first, int j,
+                                        unsigned int (&c)[8]) {
+  uint4 u[kParts];
+#pragma unroll
+  for (int r = 0; r < kParts; ++r)
+    u[r] = reinterpret_cast<const uint4*>(
+        cluster.map_shared_rank(sh->hist, (first + r) % kParts))[j];
 #pragma unroll
   for (int e = 0; e < 8; ++e) c[e] = 0;
-  for (int r = 0; r < parts; ++r) {
-    const uint4 u = reinterpret_cast<const uint4*>(cluster.map_shared_rank(sh->hist, r))[j];
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      c[2 * e] += static_cast<int>(w[e] & 0xffffu);
-      c[2 * e + 1] += static_cast<int>(w[e] >> 16);
+  for (int r = 0; r < kParts; ++r) {
+    const uint32_t w[4] = {u[r].x, u[r].y, u[r].z, u[r].w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {  // low and high half added in one instruction each
+      c[2 * e] = __dp2a_lo(w[e], 0x0001u, c[2 * e]);
+      c[2 * e + 1] = __dp2a_lo(w[e], 0x0100u, c[2 * e + 1]);
     }
   }
-}
-
-// f(index, key) over the tokens [lo, hi), 8 to a load where rows are aligned.
-template <typename F>
-__device__ __forceinline__ void each_key(const Params& p, const __half* row, int lo, int hi, F&& f) {
-  const int n8 = p.vec ? (hi - lo) >> 3 : 0;  // lo is a multiple of 8
-  for (int i = threadIdx.x; i < n8; i += kThreads) {
-    const uint4 u = *reinterpret_cast<const uint4*>(row + lo + 8 * i);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      f(lo + 8 * i + 2 * e, key_of(w[e] & 0xffffu));
-      f(lo + 8 * i + 2 * e + 1, key_of(w[e] >> 16));
-    }
-  }
-  for (int i = lo + 8 * n8 + threadIdx.x; i < hi; i += kThreads)
-    f(i, key_of(__half_as_ushort(row[i])));
 }
 
 __device__ __forceinline__ double warp_scan(double v, int lane) {  // inclusive
@@ -134,167 +198,350 @@ __device__ __forceinline__ int warp_scan(int v, int lane) {
   return v;
 }
 
-// n as a number of tokens, 1 .. c (a NaN gives 1).
-__device__ __forceinline__ int whole(double n, int c) {
-  return n >= c ? c : n > 1.0 ? static_cast<int>(n) : 1;
+__device__ __forceinline__ double warp_sum(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
 }
 
-// A place in the row's sorted order: `tokens` tokens of total mass `mass` come
-// before rank `rank` of key `key`.
+// What is asked of the sorted order. Every query holds of the first token and fails from
+// some place on: fewer than `count` tokens come before, or a mass below `mass` does
+// (up to `mass`, with `or_equal`).
+struct Query {
+  bool by_count, or_equal;
+  int count;
+  double mass;
+
+  __device__ __forceinline__ bool before(int t, double m) const {
+    return by_count ? t < count : or_equal ? m <= mass : m < mass;
+  }
+  // how many of a key's c tokens, w each, behind t tokens of mass m (1 .. c; 1 for a NaN)
+  __device__ __forceinline__ int within(int t, double m, double w, int c) const {
+    const double q = (mass - m) / w;
+    const double n = by_count ? static_cast<double>(count - t) : or_equal ? floor(q) + 1.0 : ceil(q);
+    return n >= c ? c : n > 1.0 ? static_cast<int>(n) : 1;
+  }
+};
+
+// A token of the row's sorted order: `tokens` tokens of total mass `mass` come
+// before it; it is number `rank` of key `key`'s tokens, which weigh `weight` each.
 struct Place {
   int tokens;
   double mass;
   unsigned int key;
   int rank;
+  double weight;
 };
 
-// The search of one row, by one warp of CTA 0.
+// Where several parts add up a chunk's counters, the sums stay with the part that did
+// (chunk top / 256 + i with part i mod kParts, 1 KiB each behind its Shared).
+template <int kParts>
+constexpr int kSumBytes = kParts >= 4 ? kChunks / kParts * 256 * 4 : 0;
+
+// The search of one row, by one warp of CTA 0, descending from groups of 8 chunks to
+// chunks, to 8 neighbouring keys and to a key, a lane for each. A warp alone runs at the
+// pace at which its instructions are fetched, so all queries share this code.
+template <int kParts>
 struct Search {
   cg::cluster_group& cluster;
   Shared* sh;
-  int parts, lane;
-  unsigned int top;
-  double peak, temp;
+  int lane;
+  Scale scale;
+  int group_n, group_t;   // tokens of chunks 8 lane .. 8 lane + 7, and of all before
+  double group_m;         // their mass before
 
-  // The last token whose preceding tokens satisfy `before(tokens, mass)`, a
-  // predicate that holds for nothing before and fails from some place on. Chunks,
-  // then lanes of a chunk, then keys, then tokens of a key (their number from
-  // `within(tokens, mass, weight, count)`, 1 .. count).
-  template <typename Before, typename Within>
-  __device__ Place last(Before before, Within within) const {
-    // chunk: lane holds 8 neighbouring ones
-    int tok[8], sum_t = 0;
-    double mass[8], sum_m = 0.0;
+  // Tokens and mass before every chunk; returns the row's mass.
+  __device__ __forceinline__ double prefixes() {
+    group_n = 0;
+    double m = 0.0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      tok[e] = sh->count[8 * lane + e];
-      mass[e] = sh->mass[8 * lane + e];
-      sum_t += tok[e];
-      sum_m += mass[e];
+      group_n += sh->count[8 * lane + e];
+      m += sh->mass[8 * lane + e];
     }
-    int t = warp_scan(sum_t, lane) - sum_t;
-    double m = warp_scan(sum_m, lane) - sum_m;
-    if (lane == 0) m = 0.0;
-    int best = -1, best_t = 0;
-    double best_m = 0.0;
+    group_t = warp_scan(group_n, lane) - group_n;
+    const double through = warp_scan(m, lane), all = __shfl_sync(0xffffffffu, through, 31);
+    group_m = lane == 0 ? 0.0 : through - m;
+    int t = group_t;
+    m = group_m;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      if (tok[e] > 0 && (t == 0 || before(t, m))) {
-        best = 8 * lane + e;
-        best_t = t;
-        best_m = m;
-      }
-      t += tok[e];
-      m += mass[e];
+      sh->before[8 * lane + e] = t;
+      sh->mass_before[8 * lane + e] = m;
+      t += sh->count[8 * lane + e];
+      m += sh->mass[8 * lane + e];
     }
-    const int chunk = __reduce_max_sync(0xffffffffu, best);
-    const int from = chunk >> 3;
-    best_t = __shfl_sync(0xffffffffu, best_t, from);
-    best_m = __shfl_sync(0xffffffffu, best_m, from);
-    // keys of the chunk: lane holds 8
-    int c[8];
-    double w[8];
-    counts8(cluster, sh, parts, chunk * 32 + lane, c);
-    sum_t = 0;
-    sum_m = 0.0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      w[e] = c[e] > 0 ? weight(chunk * 256 + 8 * lane + e, top, peak, temp) : 0.0;
-      sum_t += c[e];
-      sum_m += c[e] * w[e];
-    }
-    t = best_t + warp_scan(sum_t, lane) - sum_t;
-    m = best_m + (warp_scan(sum_m, lane) - sum_m);
-    if (lane == 0) m = best_m;
-    best = -1;
-    int best_c = 0;
-    double best_w = 0.0;
-    int bt = 0;
-    double bm = 0.0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if (c[e] > 0 && (t == best_t || before(t, m))) {
-        best = 8 * lane + e;
-        best_c = c[e];
-        best_w = w[e];
-        bt = t;
-        bm = m;
-      }
-      t += c[e];
-      m += c[e] * w[e];
-    }
-    const int k = __reduce_max_sync(0xffffffffu, best);
-    const int src = k >> 3;
-    bt = __shfl_sync(0xffffffffu, bt, src);
-    bm = __shfl_sync(0xffffffffu, bm, src);
-    best_c = __shfl_sync(0xffffffffu, best_c, src);
-    best_w = __shfl_sync(0xffffffffu, best_w, src);
-    const int r = min(max(within(bt, bm, best_w, best_c), 1), best_c) - 1;
-    return Place{bt + r, bm + r * best_w, static_cast<unsigned int>(chunk * 256 + k), r};
+    __syncwarp();
+    return all;
   }
 
-  // The token of rank n - 1 (n >= 1), with the mass before it.
-  __device__ Place nth(int n) const {
-    return last([=](int t, double) { return t < n; },
-                [=](int t, double, double, int) { return n - t; });
+  // The last lane that has tokens and of whose first one the query holds; it always
+  // holds of the first token of what is looked through (t == first_t).
+  __device__ __forceinline__ int pick(const Query& query, bool some, int t, double m,
+                                      int first_t) const {
+    return 31 - __clz(__ballot_sync(0xffffffffu, some && (t == first_t || query.before(t, m))));
+  }
+
+  // The last token of which the query holds.
+  __device__ __forceinline__ Place last(const Query& query) const {
+    const int group = pick(query, group_n > 0, group_t, group_m, 0);
+    // 8 chunks
+    const int at = 8 * group + (lane & 7);
+    int t = sh->before[at];
+    double m = sh->mass_before[at];
+    const int t0 = __shfl_sync(0xffffffffu, group_t, group);
+    int from = pick(query, lane < 8 && sh->count[at] > 0, t, m, t0);
+    const int chunk = 8 * group + from;
+    const int t1 = __shfl_sync(0xffffffffu, t, from);
+    const double m1 = __shfl_sync(0xffffffffu, m, from);
+    // 32 times 8 keys
+    unsigned int c[8];
+    if (kParts >= 4) {
+      const int i = chunk - static_cast<int>(scale.top >> 8);
+      const uint4* sums = reinterpret_cast<const uint4*>(
+          cluster.map_shared_rank(reinterpret_cast<uint32_t*>(sh + 1), i % kParts) +
+          i / kParts * 256 + 8 * lane);
+      const uint4 a = sums[0], b = sums[1];
+      c[0] = a.x, c[1] = a.y, c[2] = a.z, c[3] = a.w;
+      c[4] = b.x, c[5] = b.y, c[6] = b.z, c[7] = b.w;
+    } else {
+      counts8<kParts>(cluster, sh, 0, chunk * 32 + lane, c);
+    }
+    const unsigned int first = chunk * 256 + 8 * lane;
+    const double ratio = scale.ratio(first);
+    const Weights g = scale.from(first);
+    double base = g.base;
+    if (g.tiny) base = scale.exact(first);
+    int n = 0;
+    double x = 0.0;
+#pragma unroll
+    for (int e = 7; e >= 0; --e) {
+      n += c[e];
+      if (e >= g.shift) x = fma(x, ratio, as_double(c[e]));
+    }
+    x *= base;
+    t = t1 + warp_scan(n, lane) - n;
+    m = m1;
+    {
+      const double through = warp_scan(x, lane);
+      if (lane > 0) m += through - x;
+    }
+    from = pick(query, n > 0, t, m, t1);
+    // the 8 keys of that lane
+    const int t2 = __shfl_sync(0xffffffffu, t, from);
+    const double m2 = __shfl_sync(0xffffffffu, m, from);
+    base = __shfl_sync(0xffffffffu, base, from);
+    const int up = (lane & 7) - __shfl_sync(0xffffffffu, g.shift, from);
+    n = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int v = __shfl_sync(0xffffffffu, static_cast<int>(c[e]), from);
+      if (lane == e) n = v;
+    }
+    const double r2 = ratio * ratio;
+    double w = up & 1 ? base * ratio : base;
+    if (up & 2) w *= r2;
+    if (up & 4) w *= r2 * r2;
+    if (up < 0) w = 0.0;
+    x = n * w;
+    t = t2 + warp_scan(n, lane) - n;
+    m = m2;
+    {
+      const double through = warp_scan(x, lane);
+      if (lane > 0) m += through - x;
+    }
+    const int k = pick(query, n > 0, t, m, t2);
+    n = __shfl_sync(0xffffffffu, n, k);
+    t = __shfl_sync(0xffffffffu, t, k);
+    m = __shfl_sync(0xffffffffu, m, k);
+    w = __shfl_sync(0xffffffffu, w, k);
+    const int r = query.within(t, m, w, n) - 1;
+    return Place{t + r, m + r * w, static_cast<unsigned int>(chunk * 256 + 8 * from + k), r, w};
   }
 };
 
+template <int kParts>
 __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
   Shared* sh = reinterpret_cast<Shared*>(smem_raw);
   cg::cluster_group cluster = cg::this_cluster();
-  const int parts = static_cast<int>(cluster.num_blocks());
   const int part = static_cast<int>(cluster.block_rank());
-  const int64_t r = blockIdx.x / parts;
+  const int64_t r = blockIdx.x / kParts;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const __half* row = p.logits + r * p.stride;
-  const int lo = static_cast<int>(min(static_cast<int64_t>(part) * p.part, static_cast<int64_t>(p.vocab)));
+  const int lo = static_cast<int>(min(static_cast<int64_t>(part) * p.part,
+                                      static_cast<int64_t>(p.vocab)));
   const int hi = min(lo + p.part, p.vocab);
+  // tokens in front of the first 16-byte boundary, 16-byte units, tokens behind them
+  const int head = min(static_cast<int>((-reinterpret_cast<intptr_t>(row + lo) & 15) >> 1), hi - lo);
+  const int n8 = (hi - lo - head) >> 3, tail = (hi - lo - head) & 7;
+  const __half* body = row + lo + head;
+  const uint4* row8 = reinterpret_cast<const uint4*>(body);
 
   // ---- 1. histogram of this part ------------------------------------------------
+  // the row's numbers, long before they are needed
+  const float t32 = p.temperature[r], u32 = p.uniform[r];
+  const float p32 = p.top_p ? p.top_p[r] : 1.f, m32 = p.min_p ? p.min_p[r] : 0.f;
+  const int64_t k64 = p.top_k ? p.top_k[r] : 0;
+  cluster.barrier_arrive();  // (this CTA runs: the others may write its shared memory)
+  constexpr int kUnroll = 4;
+  uint4 u[kUnroll];  // the first tokens are on their way while the counters are cleared
+  auto fetch = [&](int i) {
+#pragma unroll
+    for (int k = 0; k < kUnroll; ++k)
+      if (i + k * kThreads < n8) u[k] = row8[i + k * kThreads];
+  };
+  fetch(threadIdx.x);
   for (int i = threadIdx.x; i < kKeys / 8; i += kThreads)
     reinterpret_cast<uint4*>(sh->hist)[i] = make_uint4(0, 0, 0, 0);
-  if (threadIdx.x == 0) sh->top = kKeys;
+  if (threadIdx.x < kChunks) {
+    sh->count[threadIdx.x] = sh->above[threadIdx.x] = 0;
+    sh->mass[threadIdx.x] = sh->mass_above[threadIdx.x] = 0.0;
+  }
+  if (threadIdx.x == 0) {
+    sh->top = kKeys;
+    sh->bottom = sh->some = 0;
+  }
   __syncthreads();
-  unsigned int top = kKeys;
-  each_key(p, row, lo, hi, [&](int, unsigned int key) {
-    top = min(top, key);
-    atomicAdd(&sh->hist[key >> 1], (key & 1u) ? 0x10000u : 1u);
-  });
-  top = __reduce_min_sync(0xffffffffu, top);
-  if (lane == 0) atomicMin(&sh->top, top);
-  cluster.sync();
-  for (int q = 0; q < parts; ++q) top = min(top, *cluster.map_shared_rank(&sh->top, q));
-
-  const float t32 = p.temperature[r];
-  const bool greedy = !(t32 > 0.f) || top == 0u || top >= kMinusInf;  // uniform over the cluster
-  const double peak = value_of(top), temp = static_cast<double>(t32);
-  if (!greedy) {
-    // ---- 2. tokens and mass of every chunk of keys -------------------------------
-    const double min_p = p.min_p ? static_cast<double>(p.min_p[r]) : 0.0;
-    Shared* sh0 = cluster.map_shared_rank(sh, 0);
-    for (int ch = part * (kThreads / 32) + warp; ch < kChunks; ch += parts * (kThreads / 32)) {
-      int c[8], n = 0, above = 0;
-      double m = 0.0;
-      counts8(cluster, sh, parts, ch * 32 + lane, c);
+  uint32_t top2 = 0xffffffffu, bottom2 = 0u;  // of even and odd tokens
+  auto count = [&](unsigned int key) { atomicAdd(&sh->hist[key >> 1], (key & 1u) * 0xffffu + 1u); };
+  auto count2 = [&](uint32_t bits) {
+    const uint32_t k = keys_of2(bits);
+    top2 = __vminu2(top2, k);
+    bottom2 = __vmaxu2(bottom2, k);
+    count(k & 0xffffu);
+    count(k >> 16);
+  };
+  for (int i = threadIdx.x; i < n8; i += kUnroll * kThreads) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if (c[e] > 0) {
-          const double w = weight(ch * 256 + 8 * lane + e, top, peak, temp);
-          n += c[e];
-          m += c[e] * w;
-          if (w >= min_p && w > 0.0) above += c[e];
+    for (int k = 0; k < kUnroll; ++k) {
+      if (i + k * kThreads >= n8) break;
+      count2(u[k].x);
+      count2(u[k].y);
+      count2(u[k].z);
+      count2(u[k].w);
+    }
+    fetch(i + kUnroll * kThreads);
+  }
+  if (threadIdx.x < head + tail) {
+    const int i = threadIdx.x < head ? static_cast<int>(threadIdx.x) - head
+                                     : 8 * n8 + static_cast<int>(threadIdx.x) - head;
+    const uint32_t k = keys_of2(__half_as_ushort(body[i])) & 0xffffu;
+    top2 = __vminu2(top2, 0xffff0000u | k);
+    bottom2 = __vmaxu2(bottom2, k);
+    count(k);
+  }
+  unsigned int top = __reduce_min_sync(0xffffffffu, min(top2 & 0xffffu, top2 >> 16));
+  unsigned int bottom = __reduce_max_sync(0xffffffffu, max(bottom2 & 0xffffu, bottom2 >> 16));
+  if (lane == 0) {
+    atomicMin(&sh->top, top);
+    atomicMax(&sh->bottom, bottom);
+  }
+  cluster.barrier_wait();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    // -0 counts as +0; a part with a NaN says so with key 0 at its top
+    sh->hist[kPlusZero >> 1] += (sh->hist[kMinusZero >> 1] & 0xffffu) << 16;
+    sh->hist[kMinusZero >> 1] &= 0xffff0000u;
+    if (sh->top == kMinusZero) sh->top = kPlusZero;
+    if (sh->top < kPlusInf || sh->bottom > kMinusInf) sh->top = 0;
+    for (int q = 0; q < kParts; ++q) {
+      Shared* to = cluster.map_shared_rank(sh, q);
+      to->tops[part] = sh->top;
+      to->bottoms[part] = sh->bottom;
+    }
+  }
+  cluster.sync();
+  top = kKeys;
+#pragma unroll
+  for (int q = 0; q < kParts; ++q) {
+    top = min(top, sh->tops[q]);
+    bottom = max(bottom, sh->bottoms[q]);
+  }
+
+  const bool greedy = !(t32 > 0.f) || top == 0u || top >= kMinusInf;  // uniform over the cluster
+  double step;
+  const Scale scale{top, value_of(top, step), 1.0 / static_cast<double>(t32)};
+  if (!greedy) {
+    // ---- 2. tokens and mass of every chunk of keys that occur ---------------------
+    const double min_p = static_cast<double>(m32);
+    Shared* sh0 = cluster.map_shared_rank(sh, 0);
+    // A lane sums up kGroup neighbouring keys, the lanes of a chunk together. Parts of a
+    // row on SMs of their own have warps to spare and wait for each other's counters: 8
+    // keys a lane there, a chunk a warp; 32 keys a lane, a binade a warp, else.
+    constexpr int kGroup = kParts >= 4 ? 8 : 32, kLanes = 256 / kGroup;
+#pragma unroll 1
+    for (unsigned int unit = (top >> 8) / (kGroup / 8) + part + kParts * warp;
+         unit <= (bottom >> 8) / (kGroup / 8); unit += kParts * (kThreads / 32)) {
+      const unsigned int first = (unit * 32 + lane) * kGroup;
+      const double ratio = scale.ratio(first), r2 = ratio * ratio, r4 = r2 * r2, r8 = r4 * r4;
+      const Weights g = scale.from(first, kGroup);
+      double base = g.base;
+      if (g.tiny) base = scale.exact(first);
+      const bool careful = m32 > 0.f || m32 != m32 || __any_sync(0xffffffffu, g.tiny);
+      int n = 0, above = 0;
+      double m = 0.0, ma = 0.0;
+#pragma unroll
+      for (int j = 0; j < kGroup / 8; ++j) {
+        // lanes start at different eights: rows of 64 bytes otherwise share banks
+        const int i = (j + (lane >> 1)) & (kGroup / 8 - 1);
+        unsigned int c[8];
+        counts8<kParts>(cluster, sh, part, static_cast<int>(first >> 3) + i, c);
+        if (kParts >= 4) {
+          uint4* sums = reinterpret_cast<uint4*>(reinterpret_cast<uint32_t*>(sh + 1) +
+                                                 (unit - (top >> 8)) / kParts * 256 + 8 * lane);
+          sums[0] = make_uint4(c[0], c[1], c[2], c[3]);
+          sums[1] = make_uint4(c[4], c[5], c[6], c[7]);
+        }
+        // x: weight of key 8 i of the group, then of the next keys
+        double x = base;
+        if (kGroup > 8) {
+          const int up = max(8 * i - g.shift, 0);
+          if (up & 1) x *= ratio;
+          if (up & 2) x *= r2;
+          if (up & 4) x *= r4;
+          if (up & 8) x *= r8;
+          if (up & 16) x *= r8 * r8;
+        }
+        if (!careful) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            n += c[e];
+            m = fma(as_double(c[e]), x, m);
+            if (8 * i + e >= g.shift) x *= ratio;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            n += c[e];
+            const double y = as_double(c[e]) * x;
+            m += y;
+            if (x > 0.0 && x >= min_p) {
+              above += c[e];
+              ma += y;
+            }
+            if (8 * i + e >= g.shift) x *= ratio;
+          }
         }
       }
+      if (!careful) {
+        above = n;
+        ma = m;
+      }
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
-      n = __reduce_add_sync(0xffffffffu, n);
-      above = __reduce_add_sync(0xffffffffu, above);
-      if (lane == 0) {
-        sh0->mass[ch] = m;
-        sh0->count[ch] = n;
-        sh0->above[ch] = above;
+      for (int o = kLanes / 2; o > 0; o >>= 1) {
+        m += __shfl_xor_sync(0xffffffffu, m, o);
+        ma += __shfl_xor_sync(0xffffffffu, ma, o);
+        n += __shfl_xor_sync(0xffffffffu, n, o);
+        above += __shfl_xor_sync(0xffffffffu, above, o);
+      }
+      if (lane % kLanes == 0) {
+        const int chunk = static_cast<int>(first >> 8);
+        sh0->mass[chunk] = m;
+        sh0->count[chunk] = n;
+        sh0->mass_above[chunk] = ma;
+        sh0->above[chunk] = above;
+        if (above < n) sh0->some = 1;
       }
     }
     cluster.sync();
@@ -305,75 +552,131 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
     unsigned int key = top;
     int rank = 0;
     if (!greedy) {
-      const Search s{cluster, sh, parts, lane, top, peak, temp};
-      int above = 0;
+      Search<kParts> s{cluster, sh, lane, scale};
+      // kept: tokens of the shortest prefix so far, and its mass
+      double all = s.prefixes(), mass = all;
+      int kept = p.vocab;
+      if (sh->some) {
+        kept = 0;
+        mass = 0.0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) above += sh->above[8 * lane + e];
-      int kept = max(__reduce_add_sync(0xffffffffu, above), 1);
-      const int64_t k = p.top_k ? p.top_k[r] : 0;
-      int n_k = k > 0 && k < p.vocab ? static_cast<int>(k) : p.vocab;
-      const double top_p = p.top_p ? static_cast<double>(p.top_p[r]) : 1.0;
-      if (top_p < 1.0) {
-        // mass of the top-k prefix, then the ranks whose preceding mass is below
-        // top_p of it
-        const Place z = s.nth(n_k);
-        const double all = z.mass + weight(z.key, top, peak, temp);
-        const double target = top_p * all;
-        const Place q = s.last([=](int, double m) { return m < target; },
-                               [=](int, double m, double w, int c) {
-                                 return whole(ceil((target - m) / w), c);
-                               });
-        n_k = min(n_k, q.tokens + 1);
+        for (int e = 0; e < 8; ++e) {
+          kept += sh->above[32 * e + lane];
+          mass += sh->mass_above[32 * e + lane];
+        }
+        kept = __reduce_add_sync(0xffffffffu, kept);
+        mass = warp_sum(mass);
+        if (kept == 0) {  // min_p above 1 keeps the first token all the same
+          kept = 1;
+          mass = 1.0;
+        }
       }
-      kept = min(kept, n_k);
-      const Place z = s.nth(kept);
-      const double target = static_cast<double>(p.uniform[r]) *
-                            (z.mass + weight(z.key, top, peak, temp));
-      // the last token with no more than the target before it
-      Place q = s.last([=](int, double m) { return m <= target; },
-                       [=](int, double m, double w, int c) {
-                         return whole(floor((target - m) / w) + 1.0, c);
-                       });
-      if (q.tokens >= kept) q = z;
-      key = q.key;
-      rank = q.rank;
+      // the searches in turn: 0 the end of top-k, 1 the end of top-p, 2 the last token
+      // with no more than u of the kept mass before it, 3 the last kept token when 2
+      // comes out behind it
+      Place z{};
+      for (int turn = k64 > 0 && k64 < p.vocab ? 0 : p32 < 1.f ? 1 : 2; turn < 4;) {
+        Query query{turn == 0 || turn == 3, turn == 2, turn == 0 ? static_cast<int>(k64) : kept,
+                    turn == 1 ? static_cast<double>(p32) * all : static_cast<double>(u32) * mass};
+        z = s.last(query);
+        if (turn == 0) all = z.mass + z.weight;
+        if (turn < 2 && z.tokens + 1 < kept) {
+          kept = z.tokens + 1;
+          mass = z.mass + z.weight;
+        }
+        turn = turn == 0 ? (p32 < 1.f ? 1 : 2) : turn == 1 ? 2 : turn == 2 && z.tokens >= kept ? 3 : 4;
+      }
+      key = z.key;
+      rank = z.rank;
     }
-    if (lane < parts) {
+    // tokens with that key before each part, to tell each its own rank (or that it has
+    // none); of a row with a NaN the first part that has one looks
+    int c = 0;
+    if (lane < kParts) {
+      if (key == 0) {
+        c = sh->tops[lane] == 0;
+      } else {
+        const uint32_t w = *cluster.map_shared_rank(&sh->hist[key >> 1], lane);
+        c = static_cast<int>((key & 1u) ? w >> 16 : w & 0xffffu);
+      }
+    }
+    rank -= warp_scan(c, lane) - c;
+    if (lane < kParts) {
       Shared* to = cluster.map_shared_rank(sh, lane);
       to->key = key;
-      to->rank = rank;
+      to->rank = rank < c ? rank : -1;
     }
   }
   cluster.sync();
 
-  // ---- 4. its index: the rank-th token with that key -------------------------------
+  // ---- 4. its index: the rank-th token of this part with that key -------------------
   const unsigned int key = sh->key;
   int rank = sh->rank;
-  auto counter = [&](int q) {
-    const uint32_t w = *cluster.map_shared_rank(&sh->hist[key >> 1], q);
-    return static_cast<int>((key & 1u) ? w >> 16 : w & 0xffffu);
+  if (rank < 0) return;
+  // a tile of tokens in order, one group per thread: bit e of `hit` says that token
+  // first + e of the row has the key. Counts the rank down; done below zero.
+  auto tile = [&](unsigned int hit, int first) {
+    const int n = __popc(hit), through = warp_scan(n, lane);
+    __syncthreads();  // (the last tile's sums have been read)
+    if (lane == 31) sh->warp_sum[warp] = through;
+    __syncthreads();
+    const int sum = lane < kThreads / 32 ? sh->warp_sum[lane] : 0;
+    const int before = __reduce_add_sync(0xffffffffu, lane < warp ? sum : 0);
+    const int here = rank - before - (through - n);
+    if (here >= 0 && here < n) {
+      for (int e = 0; e < here; ++e) hit &= hit - 1;
+      p.out[r] = first + __ffs(hit) - 1;
+    }
+    rank -= __reduce_add_sync(0xffffffffu, sum);
   };
-  for (int q = 0; q < part; ++q) rank -= counter(q);
-  const int own = counter(part);
-  cluster.sync();  // no CTA leaves while another reads its counters
-  if (rank < 0 || rank >= own) return;
-  // contiguous tokens per thread, in order
-  const int each = (hi - lo + kThreads - 1) / kThreads;
-  const int a = min(lo + static_cast<int>(threadIdx.x) * each, hi), z = min(a + each, hi);
-  int n = 0;
-  for (int i = a; i < z; ++i) n += key_of(__half_as_ushort(row[i])) == key;
-  int before = warp_scan(n, lane) - n;
-  if (lane == 31) sh->warp_sum[warp] = before + n;
-  __syncthreads();
-  for (int w = 0; w < warp; ++w) before += sh->warp_sum[w];
-  if (rank >= before && rank < before + n) {
-    for (int i = a; i < z; ++i) {
-      if (key_of(__half_as_ushort(row[i])) == key && before++ == rank) {
-        p.out[r] = i;
-        break;
+  auto is_key = [&](unsigned int bits) -> unsigned int { return key_of(bits & 0xffffu) == key; };
+  fetch(threadIdx.x);
+  if (head > 0)
+    tile(threadIdx.x < head && is_key(__half_as_ushort(row[lo + threadIdx.x])), lo + threadIdx.x);
+  for (int i0 = 0; i0 < n8 && rank >= 0; i0 += kUnroll * kThreads) {
+    unsigned int hit[kUnroll];
+#pragma unroll
+    for (int k = 0; k < kUnroll; ++k) {
+      hit[k] = 0;
+      if (i0 + k * kThreads + threadIdx.x < n8) {
+        const uint32_t w[4] = {u[k].x, u[k].y, u[k].z, u[k].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          hit[k] |= is_key(w[e]) << (2 * e) | is_key(w[e] >> 16) << (2 * e + 1);
       }
     }
+    fetch(i0 + kUnroll * kThreads + threadIdx.x);
+#pragma unroll
+    for (int k = 0; k < kUnroll; ++k)
+      if (rank >= 0 && i0 + k * kThreads < n8)
+        tile(hit[k], lo + head + 8 * (i0 + k * kThreads + static_cast<int>(threadIdx.x)));
   }
+  if (rank >= 0 && tail > 0) {
+    const int i = 8 * n8 + static_cast<int>(threadIdx.x);
+    tile(threadIdx.x < tail && is_key(__half_as_ushort(body[i])), lo + head + i);
+  }
+}
+
+template <int kParts>
+int launch(const Params& p, int64_t rows, int slot, cudaStream_t stream) {
+  const int st = ensure_smem_attribute(reinterpret_cast<const void*>(&sample_kernel<kParts>),
+                                       static_cast<int>(sizeof(Shared)) + kSumBytes<kParts>, slot);
+  if (st != CIE_OK) return st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = kParts;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(rows * kParts));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = sizeof(Shared) + kSumBytes<kParts>;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, sample_kernel<kParts>, p);
+  if (e != cudaSuccess) return fail(CIE_ERR_CUDA, "sample launch: %s", cudaGetErrorString(e));
+  return CIE_OK;
 }
 
 }  // namespace sample
@@ -412,25 +715,13 @@ int cie_sample_rows(const void* logits, int64_t rows, int64_t vocab, int64_t str
   p.out = out;
   p.vocab = static_cast<int>(vocab);
   p.part = static_cast<int>(part_of(parts));
-  p.vec = aligned16(logits) && stride % 8 == 0;
-  const int st = ensure_smem_attribute(reinterpret_cast<const void*>(&sample_kernel),
-                                       static_cast<int>(sizeof(Shared)), 5);
-  if (st != CIE_OK) return st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = parts;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(rows * parts));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = sizeof(Shared);
-  cfg.stream = reinterpret_cast<cudaStream_t>(stream);
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, sample_kernel, p);
-  if (e != cudaSuccess) return fail(CIE_ERR_CUDA, "sample launch: %s", cudaGetErrorString(e));
-  return CIE_OK;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  switch (parts) {
+    case 1: return launch<1>(p, rows, 5, st);
+    case 2: return launch<2>(p, rows, 6, st);
+    case 4: return launch<4>(p, rows, 7, st);
+    default: return launch<8>(p, rows, 10, st);
+  }
 }
 
 }  // extern "C"

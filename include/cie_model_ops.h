@@ -97,8 +97,8 @@ int cie_lm_head_argmax(const void* hidden, int64_t hidden_stride, const void* we
  * maximum, cie_argmax_rows' token, and so does a row that holds a NaN (its
  * first NaN). Tokens at -inf have no weight; a row of nothing else gives token
  * 0; +inf logits share all of the mass. -0 and +0 are equal. top_k (int64),
- * top_p and min_p (fp32) may be NULL (off). Rows `stride` elements apart
- * (16-byte aligned rows are read 8 values at a time). vocab <= 524224; out int64.
+ * top_p and min_p (fp32) may be NULL (off). Rows lie `stride` elements apart, at
+ * any alignment. vocab <= 524224; out int64.
  */
 int cie_sample_rows(const void* logits, int64_t rows, int64_t vocab, int64_t stride,
                     const float* uniform, const float* temperature, const int64_t* top_k,
