@@ -1,13 +1,5 @@
 // Split-KV paged GQA decode attention over 8-bit pages (sm_100a).
 //
-// One CTA per (split, sequence), eight warps; a warp takes one kv head of every
-// (8 / HKV)-th page of the split, so its working set is one K tile and one V
-// tile of 16 rows x 64 codes (1 KiB each). The tiles go from global memory
-// straight to registers, kPrefetch pages ahead. Nothing is staged in shared
-// memory, and no thread issues copies for others: half the bytes a page means
-// twice the pages a second, and one thread issuing bulk copies of 2 KiB would
-// bound the CTA (a single issuer of 4 KiB copies streams about 30 GB/s).
-//
 // Mathematics, per page and kv head (16 keys, up to 8 query heads on the MMA's N
 // side), warp-level MMA with fp16 operands and fp32 accumulation:
 //   S^T (16 x 8) = Kc (16 x 64) . Q^T (64 x 8),  s = S^T * scale_k / 8
@@ -19,13 +11,32 @@
 // ever scaled in fp16, whatever range the page scales span.
 //
 // Contraction indices and output rows may be numbered freely as long as both
-// operands agree, so every lane's operand bytes are contiguous in memory:
-//   S: lane (g, t) loads bytes [16 t, 16 t + 16) of rows pi(g) and pi(g) + 8;
+// operands agree, so every lane's operand bytes are contiguous in memory and the two
+// orders of a page's 16 rows keep shared-memory banks apart:
+//   S: lane (g, t) takes bytes [16 t, 16 t + 16) of rows pi(g) and pi(g) + 8;
 //      MMA step ks contracts dims 16 t + 4 ks + {0, 1, 2, 3}
-//   O: lane (g, t) loads bytes [8 g, 8 g + 8) of rows t, 4 + t, 8 + t, 12 + t, which
-//      are MMA keys 2t, 2t + 1, 2t + 8, 2t + 9; MMA row g of tile mt is dim 8 g + 2 mt,
-//      row g + 8 is dim 8 g + 2 mt + 1
-// with pi(2 t) = t, pi(2 t + 1) = 4 + t.
+//   O: lane (g, t) takes bytes [8 g, 8 g + 8) of rows pi(2t), pi(2t + 1), pi(2t) + 8 and
+//      pi(2t + 1) + 8, which are MMA keys 2t, 2t + 1, 2t + 8, 2t + 9; MMA row g of tile mt
+//      is dim 8 g + 2 mt, row g + 8 is dim 8 g + 2 mt + 1
+// with pi(2 t) = t, pi(2 t + 1) = 4 + (t xor 1).
+//
+// Every warp brings its own pages into its own ring of shared memory (cp.async.bulk, one
+// lane issues): half the bytes a page means twice the pages a second, and one thread
+// that issued the copies of a whole CTA would bound it (a single issuer of 4 KiB copies
+// streams about 30 GB/s).
+//
+// Work split: one CTA per (sequence, split), eight warps, each with two kv heads (or the
+// only one) of every 8th page of the split (every 4th where there are four heads). Two
+// heads a warp because their K tiles lie side by side, and so do their V tiles: with 16
+// warps per SM, scattered reads of 1 KiB stream 5.1 TB/s and of 2 KiB 6.1 TB/s on a B200.
+// The warps' results are merged in shared memory, those of several splits by a second
+// kernel.
+//
+// Measured (B200, cold pages): 256 x 4096 rows, two heads, 51 us = 5.3 TB/s, 0.81 of the
+// measured copy bandwidth; 64 x 16001-32768 80 us; one sequence of 511 rows 5.3 us, of
+// 16384 7.8 us. What bounds it: the pages' bandwidth at large sizes, with 16 warps per SM
+// (128 registers) and about 240 instructions a page and head; the chain slot -> length ->
+// block table -> page -> merge at small ones.
 #include "cie_common.cuh"
 #include "cie_host.h"
 #include "cie_kv_q8.h"
@@ -37,8 +48,20 @@ constexpr int kD = 64;
 constexpr int kPage = 16;
 constexpr int kWarps = 8;
 constexpr int kMaxGroup = 8;
-constexpr int kPrefetch = 2;
-constexpr int kAccStride = kD + 4;  // floats of one head in the merge buffer (banks)
+constexpr int kTileBytes = 2 * kPage * kD;  // K and V of one page and kv head
+constexpr int kAccStride = kD + 4;          // floats of one head in the merge buffer (banks)
+
+template <int HKV>
+struct Cfg {
+  static constexpr int kHeads = HKV == 1 ? 1 : 2;       // kv heads per warp
+  static constexpr int kStep = kWarps / (HKV / kHeads); // warps per page: pages apart
+  static constexpr int kRing = HKV == 1 ? 4 : 2;  // pages in flight per warp
+  static constexpr int kPageBytes = kHeads * kTileBytes;
+  static constexpr int kBarOffset = kWarps * kRing * kPageBytes;
+  static constexpr int kSmemBytes = kBarOffset + kWarps * kRing * 8;
+  static_assert(kRing * kPageBytes >= kHeads * kMaxGroup * kAccStride * 4,
+                "a warp's accumulators fit its ring");
+};
 
 struct Params {
   const __half* q;          // (B, H_q, D)
@@ -57,45 +80,75 @@ struct Params {
   int64_t page_stride, head_stride;
 };
 
-__device__ __forceinline__ uint4 ld_stream16(const void* p) {
-  uint4 r;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
-               : "l"(p));
-  return r;
+// `bytes` contiguous bytes from global to shared memory, counted on mbarrier `bar`.
+__device__ __forceinline__ void copy_bulk(uint32_t dst, const void* src, uint32_t bytes,
+                                          uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          dst),
+      "l"(src), "r"(bytes), "r"(bar)
+      : "memory");
 }
-
-__device__ __forceinline__ uint2 ld_stream8(const void* p) {
+__device__ __forceinline__ uint2 lds8(uint32_t addr) {
   uint2 r;
-  asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(addr) : "memory");
+  return r;
+}
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+  uint4 r;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "r"(addr)
+               : "memory");
   return r;
 }
 
-// Two biased codes of `w` (code + 128, picked by the selector) as a pair of fp16.
-__device__ __forceinline__ uint32_t codes_to_half2(uint32_t w, uint32_t sel) {
-  uint32_t h = __byte_perm(w, 0x64646464u, sel);
+// D = A(16x16, row) * B(16x8, col), fp16 inputs, fp32 accumulate.
+__device__ __forceinline__ void mma_16816_zero(float (&d)[4], uint32_t a0, uint32_t a1,
+                                               uint32_t a2, uint32_t a3, uint32_t b0,
+                                               uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
+      "{%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+// Two biased codes of `w` (code + 128, picked by the selector) as a pair of fp16; high:
+// 0x64 in every byte. It is passed in a register of its own (below): a constant that the
+// compiler may keep in a uniform register is moved from there before every use, 28
+// moves per page and head of 265 instructions.
+__device__ __forceinline__ uint32_t codes_to_half2(uint32_t w, uint32_t sel, uint32_t high) {
+  uint32_t h = __byte_perm(w, high, sel);
   const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&h), __floats2half2_rn(1152.f, 1152.f));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// One page of one kv head, as loaded.
-struct Tile {
-  uint4 k0, k1;             // rows pi(g), pi(g) + 8
-  uint2 v[4];               // rows t, 4 + t, 8 + t, 12 + t
-  float ks, vs;             // scales
-};
+__device__ __forceinline__ int seq_pages(const Params& p, int b) {
+  return decode::seq_pages(p.lens, p.slot_ids, b, p.n_slots, p.bt_stride, 0);
+}
 
 template <int HKV>
 __global__ void __launch_bounds__(32 * kWarps, 2) decode_q8_split_kernel(const Params p) {
-  constexpr int kStep = kWarps / HKV;  // warps per kv head: pages apart
-  __shared__ float s_acc[kWarps][kMaxGroup][kAccStride];
-  __shared__ float s_m[kWarps][kMaxGroup], s_l[kWarps][kMaxGroup];
+  using C = Cfg<HKV>;
+  constexpr int kHeads = C::kHeads, kStep = C::kStep, kRing = C::kRing, kThreads = 32 * kWarps;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ float2 s_ml[kWarps][kHeads][kMaxGroup];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t4 = lane & 3;
-  const int split = blockIdx.x, b = blockIdx.y, S = p.num_splits;
-  const int h = warp % HKV, par = warp / HKV;
+  const int split = blockIdx.x, b = blockIdx.y;
+  const int h0 = kHeads * (warp % (HKV / kHeads));  // this warp's first kv head
+  const int par = warp / (HKV / kHeads);
   const int H_Q = HKV * p.group;
 
+  // a page in this warp's ring: K of its heads, then V, 1 KiB each
+  const uint32_t ring = smem_u32(smem) + warp * (kRing * C::kPageBytes);
+  const uint32_t bars = smem_u32(smem + C::kBarOffset) + warp * kRing * 8;
+  if (lane == 0) {
+    for (int u = 0; u < kRing; ++u) mbar_init(bars + 8 * u, 1);
+    fence_mbar_init();
+  }
+  __syncwarp();
   // a programmatic dependent of the preceding kernel: no input is read before this
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (threadIdx.x == 0) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -111,228 +164,339 @@ __global__ void __launch_bounds__(32 * kWarps, 2) decode_q8_split_kernel(const P
     if (threadIdx.x == 0) raise_error(CIE_DEVERR_BAD_LENGTH);
     L = p.bt_stride * kPage;
   }
-  const int n_seq_pages = static_cast<int>((L + kPage - 1) / kPage);
-  const int pps = decode::split_pages(n_seq_pages, S);
+  const int Li = static_cast<int>(L), n_seq_pages = (Li + kPage - 1) / kPage;
+  const int pps = decode::split_pages(n_seq_pages, p.num_splits);
   const int page_begin = split * pps;
   const int n = max(0, min(page_begin + pps, n_seq_pages) - page_begin);
-  const int Li = static_cast<int>(L);
+  if (n == 0 && split > 0) return;  // (split 0 writes a zero row)
   const int mine = n > par ? (n - par + kStep - 1) / kStep : 0;  // pages of this warp
 
-  // Page ids and scales of 32 of this warp's pages at a time, one per lane: the
-  // batch in use, the ids of the next one (whose scales are on their way) and the
-  // table entries of the one after.
-  const int64_t bt_row = slot * p.bt_stride + page_begin;
+  // Page ids and scales of 32 of this warp's pages at a time, one per lane (the block-table
+  // entries of the next 32 on their way). Scales: ks times head_dim ** -0.5 * log2(e).
+  const int64_t bt_row = slot * p.bt_stride + page_begin + par;
   auto entry = [&](int i) -> int64_t {
-    return i < mine ? p.table.at(bt_row + par + static_cast<int64_t>(i) * kStep) : 0;
+    return i < mine ? p.table.at(bt_row + static_cast<int64_t>(i) * kStep) : 0;
   };
-  auto checked = [&](int64_t pid) -> int {
-    if (pid < 0 || pid >= p.n_pages) {
-      raise_error(CIE_DEVERR_BAD_PAGE);
-      return 0;
-    }
-    return static_cast<int>(pid);
-  };
-  int pid_c = 0, pid_n = 0;
-  float ks_c = 0.f, vs_c = 0.f, ks_n = 0.f, vs_n = 0.f;
-  int64_t e_nn = 0;
-  auto load_scales = [&](int pid, float& ks, float& vs) {
-    const float* sp = p.scales + static_cast<int64_t>(pid) * (2 * HKV) + h;
-    ks = sp[0];
-    vs = sp[HKV];
-  };
-
-  Tile tile[kPrefetch];
-  auto fetch = [&](Tile& x, int i) {  // page i of this warp; i counts up from 0
+  int64_t entry_n = entry(lane);
+  int pid = 0;
+  float ks[kHeads], vs[kHeads], ks_n[kHeads], vs_n[kHeads];
+  const int8_t* k_base = p.k + h0 * p.head_stride;
+  const int8_t* v_base = p.v + h0 * p.head_stride;
+  int put = 0;  // ring place of the next page to fetch
+  auto fetch = [&](int i) {
     if (i >= mine) return;
-    if (i != 0 && (i & 31) == 0) {
-      pid_c = pid_n;
-      ks_c = ks_n;
-      vs_c = vs_n;
-      pid_n = checked(e_nn);
-      load_scales(pid_n, ks_n, vs_n);
-      e_nn = entry(i + 64 + lane);
+    if ((i & 31) == 0) {
+      if (entry_n < 0 || entry_n >= p.n_pages) {
+        raise_error(CIE_DEVERR_BAD_PAGE);
+        entry_n = 0;
+      }
+      pid = static_cast<int>(entry_n);
     }
-    const int pid = __shfl_sync(0xffffffffu, pid_c, i & 31);
-    x.ks = __shfl_sync(0xffffffffu, ks_c, i & 31);
-    x.vs = __shfl_sync(0xffffffffu, vs_c, i & 31);
-    const int64_t at = static_cast<int64_t>(pid) * p.page_stride + h * p.head_stride;
-    const int8_t* kp = p.k + at + ((g >> 1) + 4 * (g & 1)) * kD + 16 * t4;
-    x.k0 = ld_stream16(kp);
-    x.k1 = ld_stream16(kp + 8 * kD);
-    const int8_t* vp = p.v + at + t4 * kD + 8 * g;
+    const int64_t at = __shfl_sync(0xffffffffu, pid, i & 31) * p.page_stride;
+    if (lane == 0) {
+      const uint32_t to = ring + put * C::kPageBytes, bar = bars + 8 * put;
+      mbar_arrive_expect_tx(bar, C::kPageBytes);
+      if (p.head_stride == kPage * kD) {  // the heads of a page lie side by side
+        copy_bulk(to, k_base + at, C::kPageBytes / 2, bar);
+        copy_bulk(to + C::kPageBytes / 2, v_base + at, C::kPageBytes / 2, bar);
+      } else {
+        for (int u = 0; u < kHeads; ++u) {
+          copy_bulk(to + 1024 * u, k_base + at + u * p.head_stride, 1024, bar);
+          copy_bulk(to + 1024 * (kHeads + u), v_base + at + u * p.head_stride, 1024, bar);
+        }
+      }
+    }
+    put = put + 1 == kRing ? 0 : put + 1;
+    if ((i & 31) == 0) {
+      const float* sp = p.scales + static_cast<int64_t>(pid) * (2 * HKV) + h0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x.v[j] = ld_stream8(vp + 4 * j * kD);
+      for (int u = 0; u < kHeads; ++u) {
+        ks_n[u] = sp[u] * (0.125f * kLog2e);
+        vs_n[u] = sp[HKV + u];
+      }
+      entry_n = entry(i + 32 + lane);
+    }
   };
-  if (mine > 0) {
-    pid_c = checked(entry(lane));
-    load_scales(pid_c, ks_c, vs_c);
-    pid_n = checked(entry(32 + lane));
-    load_scales(pid_n, ks_n, vs_n);
-    e_nn = entry(64 + lane);
-#pragma unroll
-    for (int u = 0; u < kPrefetch; ++u) fetch(tile[u], u);
-  }
+#pragma unroll 1
+  for (int u = 0; u < kRing; ++u) fetch(u);
 
-  // Q^T as the B operand: lane (g, t) holds query head g, dims 16 t .. 16 t + 15
-  uint32_t bq[4][2];
+  uint32_t bq[kHeads][4][2];
+  float m[kHeads][2], l[kHeads][2];  // query heads 2 t, 2 t + 1 of each kv head; m in log2
+  float acc[kHeads][4][4];
+
   {
-    const bool valid = g < p.group;
-    const uint4* qr = reinterpret_cast<const uint4*>(
-        p.q + (static_cast<int64_t>(b) * H_Q + h * p.group + (valid ? g : 0)) * kD + 16 * t4);
-    const uint4 a = valid ? qr[0] : make_uint4(0, 0, 0, 0);
-    const uint4 c = valid ? qr[1] : make_uint4(0, 0, 0, 0);
-    bq[0][0] = a.x;
-    bq[0][1] = a.y;
-    bq[1][0] = a.z;
-    bq[1][1] = a.w;
-    bq[2][0] = c.x;
-    bq[2][1] = c.y;
-    bq[3][0] = c.z;
-    bq[3][1] = c.w;
+          // Q^T as the B operand: lane (g, t) holds query head g, dims 16 t .. 16 t + 15
+          const bool valid = g < p.group;
+    #pragma unroll
+          for (int u = 0; u < kHeads; ++u) {
+            const uint4* qr = reinterpret_cast<const uint4*>(
+                p.q + (static_cast<int64_t>(b) * H_Q + (h0 + u) * p.group + (valid ? g : 0)) * kD +
+                16 * t4);
+            const uint4 a = valid ? qr[0] : make_uint4(0, 0, 0, 0);
+            const uint4 d = valid ? qr[1] : make_uint4(0, 0, 0, 0);
+            bq[u][0][0] = a.x;
+            bq[u][0][1] = a.y;
+            bq[u][1][0] = a.z;
+            bq[u][1][1] = a.w;
+            bq[u][2][0] = d.x;
+            bq[u][2][1] = d.y;
+            bq[u][3][0] = d.z;
+            bq[u][3][1] = d.w;
+            m[u][0] = m[u][1] = -CUDART_INF_F;
+            l[u][0] = l[u][1] = 0.f;
+    #pragma unroll
+            for (int e = 0; e < 16; ++e) acc[u][e >> 2][e & 3] = 0.f;
+          }
+  }
+  uint32_t high;
+  asm volatile("mov.u32 %0, %%laneid;" : "=r"(high));
+  high = (high >> 5) + 0x64646464u;  // laneid < 32
+  // rows pi(g), pi(2 t) and pi(2 t + 1), and this lane's bytes of them
+  const int row_g = g & 1 ? 4 + ((g >> 1) ^ 1) : g >> 1;
+  const uint32_t k_at = ring + row_g * kD + 16 * t4;
+  const uint32_t v_at = ring + kHeads * 1024 + t4 * kD + 8 * g;
+  const uint32_t v_odd = (4 + (t4 ^ 1) - t4) * kD;  // from row pi(2 t) to row pi(2 t + 1)
+  int get = 0;  // ring place of page i
+  uint32_t phase = 0;
+#pragma unroll 1
+  for (int i = 0; i < mine; ++i) {
+    if (!__all_sync(0xffffffffu, mbar_wait(bars + 8 * get, phase, CIE_DEVERR_WAIT_TIMEOUT))) {
+      // gave up: leave no copy in flight (each wait is bounded)
+      for (int j = i; j < min(i + kRing, mine); ++j) {
+        mbar_wait(bars + 8 * get, phase, CIE_DEVERR_WAIT_TIMEOUT);
+        get = get + 1 == kRing ? 0 : get + 1;
+        if (get == 0) phase ^= 1;
+      }
+      break;
+    }
+    if ((i & 31) == 0) {  // (fetch is less than 32 pages ahead)
+#pragma unroll
+      for (int u = 0; u < kHeads; ++u) {
+        ks[u] = ks_n[u];
+        vs[u] = vs_n[u];
+      }
+    }
+    const uint32_t page = get * C::kPageBytes;
+
+    // scores (times log2 e): keys pi(g), pi(g) + 8 of query heads 2 t, 2 t + 1
+    float s[kHeads][4];
+#pragma unroll
+    for (int u = 0; u < kHeads; ++u) {
+      const uint4 k0 = lds16(k_at + page + 1024 * u), k1 = lds16(k_at + page + 1024 * u + 512);
+      const uint32_t* kw0 = reinterpret_cast<const uint32_t*>(&k0);
+      const uint32_t* kw1 = reinterpret_cast<const uint32_t*>(&k1);
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        const uint32_t w0 = kw0[ks] ^ 0x80808080u, w1 = kw1[ks] ^ 0x80808080u;
+        const uint32_t a0 = codes_to_half2(w0, 0x4140, high), a1 = codes_to_half2(w1, 0x4140, high);
+        const uint32_t a2 = codes_to_half2(w0, 0x4342, high), a3 = codes_to_half2(w1, 0x4342, high);
+        if (ks == 0) mma_16816_zero(s[u], a0, a1, a2, a3, bq[u][0][0], bq[u][0][1]);
+        else mma_16816(s[u], a0, a1, a2, a3, bq[u][ks][0], bq[u][ks][1]);
+      }
+    }
+    float kf[kHeads], vf[kHeads];
+#pragma unroll
+    for (int u = 0; u < kHeads; ++u) {
+      kf[u] = __shfl_sync(0xffffffffu, ks[u], i & 31);
+      vf[u] = __shfl_sync(0xffffffffu, vs[u], i & 31);
+    }
+    const int rows = Li - (page_begin + par + i * kStep) * kPage;  // visible, if below 16
+    float al[kHeads][2];
+    bool grew = false;
+#pragma unroll
+    for (int u = 0; u < kHeads; ++u) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[u][e] *= kf[u];
+      if (rows < kPage) {  // rows behind the sequence's end
+        if (row_g >= rows) s[u][0] = s[u][1] = -CUDART_INF_F;
+        if (row_g + 8 >= rows) s[u][2] = s[u][3] = -CUDART_INF_F;
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        // row 0 of a page is always visible, so the new maximum is finite
+        const float mn = fmaxf(m[u][e], decode::shfl_max_group(fmaxf(s[u][e], s[u][2 + e])));
+        grew |= mn != m[u][e];
+        al[u][e] = m[u][e] - mn;
+        m[u][e] = mn;
+      }
+    }
+    if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+      for (int u = 0; u < kHeads; ++u) {
+        const float a0 = ex2(al[u][0]), a1 = ex2(al[u][1]);
+        l[u][0] *= a0;
+        l[u][1] *= a1;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          acc[u][t][0] *= a0;
+          acc[u][t][1] *= a1;
+          acc[u][t][2] *= a0;
+          acc[u][t][3] *= a1;
+        }
+      }
+    }
+    uint32_t pb[kHeads][2];
+#pragma unroll
+    for (int u = 0; u < kHeads; ++u) {
+      const float p0 = ex2(s[u][0] - m[u][0]), p1 = ex2(s[u][1] - m[u][1]);
+      const float p2 = ex2(s[u][2] - m[u][0]), p3 = ex2(s[u][3] - m[u][1]);
+      l[u][0] += p0 + p2;
+      l[u][1] += p1 + p3;
+      pb[u][0] = movmatrix_trans(pack_half2(p0, p1));
+      pb[u][1] = movmatrix_trans(pack_half2(p2, p3));
+    }
+    // acc += scale_v * V^T . P^T
+#pragma unroll
+    for (int u = 0; u < kHeads; ++u) {
+      const uint32_t va = v_at + page + 1024 * u;
+      const uint2 v0 = lds8(va), v1 = lds8(va + v_odd), v2 = lds8(va + 512), v3 = lds8(va + 512 + v_odd);
+#pragma unroll
+      for (int wd = 0; wd < 2; ++wd) {  // dims 8 g + 4 wd .. + 3: MMA tiles 2 wd, 2 wd + 1
+        const uint32_t ra = (wd ? v0.y : v0.x) ^ 0x80808080u;
+        const uint32_t rb = (wd ? v1.y : v1.x) ^ 0x80808080u;
+        const uint32_t rc = (wd ? v2.y : v2.x) ^ 0x80808080u;
+        const uint32_t rd = (wd ? v3.y : v3.x) ^ 0x80808080u;
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {  // dims 2 hf, 2 hf + 1 of the word
+          const uint32_t sel = hf ? 0x7362 : 0x5140;  // bytes of one dim side by side
+          const uint32_t ab = __byte_perm(ra, rb, sel), cd = __byte_perm(rc, rd, sel);
+          float o[4];
+          mma_16816_zero(o, codes_to_half2(ab, 0x4140, high), codes_to_half2(ab, 0x4342, high),
+                         codes_to_half2(cd, 0x4140, high), codes_to_half2(cd, 0x4342, high), pb[u][0], pb[u][1]);
+          float* d = acc[u][2 * wd + hf];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) d[e] = fmaf(o[e], vf[u], d[e]);
+        }
+      }
+    }
+    __syncwarp();  // the page has been read
+    fetch(i + kRing);
+    get = get + 1 == kRing ? 0 : get + 1;
+    if (get == 0) phase ^= 1;
   }
 
-  float m0 = -CUDART_INF_F, m1 = -CUDART_INF_F;  // heads 2 t, 2 t + 1
-  float l0 = 0.f, l1 = 0.f;
-  float acc[4][4];
-#pragma unroll
-  for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[mt][e] = 0.f;
-
-  auto step = [&](const Tile& x, int i) {
-    float sc[4] = {0.f, 0.f, 0.f, 0.f};
-    const uint32_t* kw0 = reinterpret_cast<const uint32_t*>(&x.k0);
-    const uint32_t* kw1 = reinterpret_cast<const uint32_t*>(&x.k1);
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      const uint32_t w0 = kw0[ks] ^ 0x80808080u, w1 = kw1[ks] ^ 0x80808080u;
-      mma_16816(sc, codes_to_half2(w0, 0x4140), codes_to_half2(w1, 0x4140),
-                codes_to_half2(w0, 0x4342), codes_to_half2(w1, 0x4342), bq[ks][0], bq[ks][1]);
-    }
-    const float f = x.ks * 0.125f;  // head_dim ** -0.5 for D = 64
-    float s0 = sc[0] * f, s1 = sc[1] * f, s2 = sc[2] * f, s3 = sc[3] * f;
-    const int first = (page_begin + par + i * kStep) * kPage;
-    if (first + kPage > Li) {  // the sequence's last page: rows beyond its end
-      const int key0 = first + (g >> 1) + 4 * (g & 1);
-      if (key0 >= Li) s0 = s1 = -CUDART_INF_F;
-      if (key0 + 8 >= Li) s2 = s3 = -CUDART_INF_F;
-    }
-    const float mn0 = fmaxf(m0, decode::shfl_max_group(fmaxf(s0, s2)));
-    const float mn1 = fmaxf(m1, decode::shfl_max_group(fmaxf(s1, s3)));
-    if (__any_sync(0xffffffffu, mn0 != m0 || mn1 != m1)) {
-      // row 0 of a visited page is always visible, so mn0 and mn1 are finite here
-      const float al0 = ex2((m0 - mn0) * kLog2e);
-      const float al1 = ex2((m1 - mn1) * kLog2e);
-      l0 *= al0;
-      l1 *= al1;
-#pragma unroll
-      for (int mt = 0; mt < 4; ++mt) {
-        acc[mt][0] *= al0;
-        acc[mt][1] *= al1;
-        acc[mt][2] *= al0;
-        acc[mt][3] *= al1;
-      }
-      m0 = mn0;
-      m1 = mn1;
-    }
-    const float p0 = ex2((s0 - m0) * kLog2e);
-    const float p1 = ex2((s1 - m1) * kLog2e);
-    const float p2 = ex2((s2 - m0) * kLog2e);
-    const float p3 = ex2((s3 - m1) * kLog2e);
-    l0 += p0 + p2;
-    l1 += p1 + p3;
-    const uint32_t pb0 = movmatrix_trans(pack_half2(p0, p1));
-    const uint32_t pb1 = movmatrix_trans(pack_half2(p2, p3));
-#pragma unroll
-    for (int wd = 0; wd < 2; ++wd) {  // dims 8 g + 4 wd .. + 3: MMA tiles 2 wd, 2 wd + 1
-      const uint32_t ra = (wd ? x.v[0].y : x.v[0].x) ^ 0x80808080u;
-      const uint32_t rb = (wd ? x.v[1].y : x.v[1].x) ^ 0x80808080u;
-      const uint32_t rc = (wd ? x.v[2].y : x.v[2].x) ^ 0x80808080u;
-      const uint32_t rd = (wd ? x.v[3].y : x.v[3].x) ^ 0x80808080u;
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {  // dims 2 hf, 2 hf + 1 of the word
-        const uint32_t sel = hf ? 0x7362 : 0x5140;  // bytes of one dim side by side
-        const uint32_t ab = __byte_perm(ra, rb, sel), cd = __byte_perm(rc, rd, sel);
-        float o[4] = {0.f, 0.f, 0.f, 0.f};
-        mma_16816(o, codes_to_half2(ab, 0x4140), codes_to_half2(ab, 0x4342),
-                  codes_to_half2(cd, 0x4140), codes_to_half2(cd, 0x4342), pb0, pb1);
-        float* d = acc[2 * wd + hf];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) d[e] = fmaf(o[e], x.vs, d[e]);
-      }
-    }
+  // ---- the warps' results, merged ---------------------------------------------------
+  __syncwarp();
+  auto acc_of = [&](int w, int u, int hh) {  // accumulator rows in the rings
+    return reinterpret_cast<float*>(smem + w * (kRing * C::kPageBytes)) +
+           (u * kMaxGroup + hh) * kAccStride;
   };
-
-  for (int i = 0; i < mine; i += kPrefetch) {
 #pragma unroll
-    for (int u = 0; u < kPrefetch; ++u) {
-      if (i + u < mine) step(tile[u], i + u);
-      fetch(tile[u], i + u + kPrefetch);
+  for (int u = 0; u < kHeads; ++u) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {  // query head 2 t + e, dims 8 g .. 8 g + 7
+      const float sum = decode::shfl_sum_group(l[u][e]);
+      float4* d = reinterpret_cast<float4*>(acc_of(warp, u, 2 * t4 + e) + 8 * g);
+      d[0] = make_float4(acc[u][0][e], acc[u][0][2 + e], acc[u][1][e], acc[u][1][2 + e]);
+      d[1] = make_float4(acc[u][2][e], acc[u][2][2 + e], acc[u][3][e], acc[u][3][2 + e]);
+      if (g == 0) s_ml[warp][u][2 * t4 + e] = make_float2(m[u][e], sum);
     }
-  }
-  l0 = decode::shfl_sum_group(l0);
-  l1 = decode::shfl_sum_group(l1);
-
-  // ---- the warps of a kv head, merged -----------------------------------------
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {  // heads 2 t + e, dims 8 g .. 8 g + 7
-    float4* d = reinterpret_cast<float4*>(&s_acc[warp][2 * t4 + e][8 * g]);
-    d[0] = make_float4(acc[0][e], acc[0][2 + e], acc[1][e], acc[1][2 + e]);
-    d[1] = make_float4(acc[2][e], acc[2][2 + e], acc[3][e], acc[3][2 + e]);
-  }
-  if (g == 0) {
-    s_m[warp][2 * t4] = m0;
-    s_m[warp][2 * t4 + 1] = m1;
-    s_l[warp][2 * t4] = l0;
-    s_l[warp][2 * t4 + 1] = l1;
   }
   __syncthreads();
-  if (S > 1 && n == 0) return;  // the merge reads only splits that saw pages
-  for (int i = threadIdx.x; i < HKV * p.group * (kD / 4); i += 32 * kWarps) {
+  for (int i = threadIdx.x; i < H_Q * (kD / 4); i += kThreads) {
     const int hq = i / (kD / 4), d4 = i % (kD / 4);
-    const int kv = hq / p.group, hh = hq % p.group;
+    const int kv = hq / p.group, hh = hq - kv * p.group, u = kv % kHeads, w0 = kv / kHeads;
+    float2 ml[kStep];
     float M = -CUDART_INF_F;
 #pragma unroll
-    for (int w = 0; w < kStep; ++w) M = fmaxf(M, s_m[w * HKV + kv][hh]);
-    float l = 0.f;
+    for (int w = 0; w < kStep; ++w) {
+      ml[w] = s_ml[w * (HKV / kHeads) + w0][u][hh];
+      M = fmaxf(M, ml[w].x);
+    }
+    float sum = 0.f;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (M != -CUDART_INF_F) {
+    if (n > 0) {
 #pragma unroll
       for (int w = 0; w < kStep; ++w) {
-        const float wt = ex2((s_m[w * HKV + kv][hh] - M) * kLog2e);
-        const float4 x = *reinterpret_cast<const float4*>(&s_acc[w * HKV + kv][hh][4 * d4]);
-        l += wt * s_l[w * HKV + kv][hh];
+        const float wt = ex2(ml[w].x - M);  // 0 of a warp that saw no page
+        const float4 x = *reinterpret_cast<const float4*>(
+            acc_of(w * (HKV / kHeads) + w0, u, hh) + 4 * d4);
+        sum += wt * ml[w].y;
         a.x += wt * x.x;
         a.y += wt * x.y;
         a.z += wt * x.z;
         a.w += wt * x.w;
       }
     }
-    if (S == 1) {
-      const float inv = l > 0.f ? 1.f / l : 0.f;  // a row that saw no key is zero
+    if (n == n_seq_pages) {
+      const float inv = n > 0 ? 1.f / sum : 0.f;  // a row that saw no key is zero
       uint2 r;
       r.x = pack_half2(a.x * inv, a.y * inv);
       r.y = pack_half2(a.z * inv, a.w * inv);
       *reinterpret_cast<uint2*>(p.o + (static_cast<int64_t>(b) * H_Q + hq) * kD + 4 * d4) = r;
     } else {
-      const int64_t row = (static_cast<int64_t>(b) * S + split) * H_Q + hq;
+      const int64_t row = (static_cast<int64_t>(b) * p.num_splits + split) * H_Q + hq;
       *reinterpret_cast<float4*>(p.ws_acc + row * kD + 4 * d4) = a;
-      if (d4 == 0) {
-        p.ws_ml[row * 2] = M;
-        p.ws_ml[row * 2 + 1] = l;
-      }
+      if (d4 == 0) *reinterpret_cast<float2*>(p.ws_ml + row * 2) = make_float2(M, sum);
     }
   }
 }
 
+// Merges the partials of the sequences that have several splits: O = sum_s w_s acc_s /
+// sum_s w_s l_s, w_s = 2^(m_s - max m). kFold > 1: a CTA of kFold warps per (query head,
+// sequence), each folding every kFold-th split; 1: a CTA per sequence, a warp per query
+// head. A lane holds two columns. A programmatic dependent of the split kernel.
+template <int HKV, int kFold>
+__global__ void __launch_bounds__(kFold > 1 ? 32 * kFold : 1024) merge_q8_kernel(const Params p) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int H_Q = HKV * p.group;
+  const int b = blockIdx.x, hq = kFold > 1 ? blockIdx.y : warp, fold = kFold > 1 ? warp : 0;
+  // (the split kernel does not write slots and lengths)
+  const int n = seq_pages(p, b);
+  const int pps = decode::split_pages(n, p.num_splits);
+  if (n <= pps) return;
+  const int splits = (n + pps - 1) / pps;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  float M = -CUDART_INF_F, l = 0.f;
+  float2 acc = make_float2(0.f, 0.f);
+#pragma unroll 4
+  for (int s = fold; s < splits; s += kFold) {
+    const int64_t row = (static_cast<int64_t>(b) * p.num_splits + s) * H_Q + hq;
+    const float2 ml = *reinterpret_cast<const float2*>(p.ws_ml + row * 2);
+    const float2 a = *reinterpret_cast<const float2*>(p.ws_acc + row * kD + 2 * lane);
+    const float Mn = fmaxf(M, ml.x);  // finite: every split saw a key
+    const float wo = ex2(M - Mn), wn = ex2(ml.x - Mn);
+    l = l * wo + ml.y * wn;
+    acc.x = acc.x * wo + a.x * wn;
+    acc.y = acc.y * wo + a.y * wn;
+    M = Mn;
+  }
+  if (kFold > 1) {
+    __shared__ float s_m[kFold], s_l[kFold];
+    __shared__ float2 s_acc[kFold][32];
+    if (lane == 0) {
+      s_m[fold] = M;
+      s_l[fold] = l;
+    }
+    s_acc[fold][lane] = acc;
+    __syncthreads();
+    if (fold != 0) return;
+    for (int w = 1; w < min(kFold, splits); ++w) {
+      const float Mn = fmaxf(M, s_m[w]);
+      const float wo = ex2(M - Mn), wn = ex2(s_m[w] - Mn);
+      l = l * wo + s_l[w] * wn;
+      acc.x = acc.x * wo + s_acc[w][lane].x * wn;
+      acc.y = acc.y * wo + s_acc[w][lane].y * wn;
+      M = Mn;
+    }
+  }
+  const float inv = 1.f / l;
+  *reinterpret_cast<__half2*>(p.o + (static_cast<int64_t>(b) * H_Q + hq) * kD + 2 * lane) =
+      __floats2half2_rn(acc.x * inv, acc.y * inv);
+}
+
 template <int HKV>
 int launch(const Params& p, int batch, cudaStream_t stream) {
+  const int st = ensure_smem_attribute(reinterpret_cast<const void*>(&decode_q8_split_kernel<HKV>),
+                                       Cfg<HKV>::kSmemBytes, 10 + HKV);
+  if (st != CIE_OK) return st;
   cudaLaunchAttribute pdl[1];
   pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   pdl[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(p.num_splits, batch);
   cfg.blockDim = dim3(32 * kWarps);
+  cfg.dynamicSmemBytes = Cfg<HKV>::kSmemBytes;
   cfg.stream = stream;
   cfg.attrs = pdl;
   cfg.numAttrs = 1;
@@ -340,14 +504,12 @@ int launch(const Params& p, int batch, cudaStream_t stream) {
   if (e != cudaSuccess) return fail(CIE_ERR_CUDA, "decode_q8 launch: %s", cudaGetErrorString(e));
   if (p.num_splits > 1) {
     const int H_Q = HKV * p.group;
-    const bool small = p.num_splits <= decode::kSmallMergeSplits;
-    cfg.gridDim = small ? dim3(batch) : dim3(H_Q, batch);
-    cfg.blockDim = dim3(small ? 32 * H_Q : 256);
-    e = cudaLaunchKernelEx(&cfg,
-                           small ? decode::decode_merge_small_kernel : decode::decode_merge_kernel,
-                           static_cast<const float*>(p.ws_acc),
-                           static_cast<const float*>(p.ws_ml), p.o, p.lens, p.slot_ids,
-                           p.n_slots, p.bt_stride, p.num_splits, H_Q, 0);
+    const bool wide = p.num_splits > 16;  // few sequences, many splits
+    cfg.gridDim = wide ? dim3(batch, H_Q) : dim3(batch);
+    cfg.blockDim = dim3(wide ? 256 : 32 * H_Q);
+    cfg.dynamicSmemBytes = 0;
+    e = wide ? cudaLaunchKernelEx(&cfg, merge_q8_kernel<HKV, 8>, p)
+             : cudaLaunchKernelEx(&cfg, merge_q8_kernel<HKV, 1>, p);
     if (e != cudaSuccess) return fail(CIE_ERR_CUDA, "merge launch: %s", cudaGetErrorString(e));
   }
   return CIE_OK;
@@ -417,7 +579,21 @@ int entry(const void* q, const void* k, const void* v, const float* kv_scales,
 extern "C" {
 
 int cie_decode_q8_default_splits(int batch, int device) {
-  return cie_decode_default_splits(batch, device);
+  int sms = 148;
+  if (device >= 0) {
+    int n = 0;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) == cudaSuccess && n > 0)
+      sms = n;
+  }
+  if (batch <= 0) return 1;
+  // Two CTAs per SM, as the smallest power of two that is at least 4/5 of that. More CTAs
+  // even out ragged batches, where the longest split sets the time (256 sequences of 1 to
+  // 4096 rows, one kv head: 29.1 us at 1 split, 21.7 at 2, 25.7 at 4; 100 of 1 to 4000,
+  // four heads: 39.0 at 2, 26.4 at 4), but cost even ones a second wave and a merge
+  // (256 x 4096, two heads: 49.8 us at 1 split, 55.2 at 2; 64 x 4096: 18.6 at 4, 20.4 at 8).
+  int s = 1;
+  while (s < 64 && 5LL * s * batch < 8LL * sms) s *= 2;
+  return s;
 }
 
 int cie_decode_attention_q8(const void* q, const void* k, const void* v, const float* kv_scales,
