@@ -37,6 +37,9 @@ rope_kv_decode_update_op = torch.ops.inference.rope_kv_decode_update.default
 rope_kv_mixed_update_op = torch.ops.inference.rope_kv_mixed_update.default
 rope_kv_decode_attention_op = torch.ops.inference.rope_kv_decode_attention.default
 rope_kv_mixed_attention_op = torch.ops.inference.rope_kv_mixed_attention.default
+rope_kv_q8_decode_update_op = torch.ops.inference.rope_kv_q8_decode_update.default
+rope_kv_q8_mixed_update_op = torch.ops.inference.rope_kv_q8_mixed_update.default
+gqa_decode_attention_q8_op = torch.ops.inference.gqa_decode_attention_q8.default
 _gqa_decode_attention_splits = torch.ops.inference.gqa_decode_attention_splits.default
 
 # The reference tunes Triton tiles here (attn/core.py:114-116). The CUDA decode
@@ -114,6 +117,9 @@ class TritonQwen2Attention(torch.nn.Module):
     reference's modules never sets it, because the reference's piecewise
     backend splits the graph at ``inference::gqa_mixed_attention`` nodes
     (piecewise/utils.py:5-23), which the one-call form does not contain.
+    Over a ``QuantizedKVStorage`` both passes rotate, quantise and write in one
+    launch; a decode pass then attends to the 8-bit pages, a mixed pass reads its
+    histories back to fp16 pages and runs the mixed attention op on those.
     Without ``kv_manager`` it defers to the wrapped HF module.
     """
 
@@ -155,6 +161,9 @@ class TritonQwen2Attention(torch.nn.Module):
         qkv = torch.nn.functional.linear(hidden_states, self.qkv_weight, self.qkv_bias)
         cos, sin = position_embeddings
         layer = self.layer_idx
+        if getattr(kv_manager, "quantized", False):
+            o = self._quantized_attention(qkv, cos, sin, kv_manager, metadata)
+            return self.original.o_proj(o.reshape(1, total_T, self.num_heads * self.head_dim)), None
         if self.fuse_rope and self.fuse_decode_attention and metadata.full_decode:
             # RoPE, K/V write and decode attention: one launch
             o = rope_kv_decode_attention_op(qkv, cos, sin, kv_manager.keys[layer],
@@ -209,6 +218,45 @@ class TritonQwen2Attention(torch.nn.Module):
                                        block_table=kv_manager.block_table)
         out = self.original.o_proj(o.reshape(1, total_T, self.num_heads * self.head_dim))
         return out, None
+
+
+    def _quantized_attention(self, qkv, cos, sin, kv, metadata):
+        """Write and attention of one pass over 8-bit pages."""
+        layer, pool = self.layer_idx, kv.pool(self.layer_idx)
+        slots, table = metadata.slot_ids, kv.block_table
+        lens = getattr(metadata, "attn_lens", None)
+        if metadata.full_decode:
+            if lens is None:
+                lens = kv.lens[slots] + 1
+            if self.fuse_rope:
+                q = rope_kv_q8_decode_update_op(qkv, cos, sin, *pool, kv.lens, slots, table)
+            else:
+                q, k, v = self._rotated(qkv, cos, sin)
+                kv.decode_update(layer, slots, k, v)
+            return gqa_decode_attention_q8_op(q, *pool, lens, slots, table)
+        if lens is None:
+            lens = kv.lens[slots]
+        cu = metadata.cu_seqlens
+        ends = getattr(metadata, "read_lens", None)
+        if ends is None:
+            ends = lens + cu[1:] - cu[:-1]
+        if self.fuse_rope:
+            q = rope_kv_q8_mixed_update_op(qkv, cos, sin, *pool, cu, lens, slots, table)
+        else:
+            q, k, v = self._rotated(qkv, cos, sin)
+            kv.mixed_update_sequences(layer, cu, lens, slots, k, v)
+        keys, values = kv.read(layer, slots, ends)
+        return gqa_mixed_attention_op(q, keys, values, kv_lens=lens,
+                                      max_seqlen=metadata.max_seqlen, cu_seqlens=cu,
+                                      slot_ids=slots, block_table=table)
+
+    def _rotated(self, qkv, cos, sin):
+        from transformers.models.qwen2.modeling_qwen2 import apply_rotary_pos_emb
+
+        shape = (1, qkv.shape[1], -1, self.head_dim)
+        q, k, v = qkv.split(self.qkv_sizes, dim=-1)
+        q, k = apply_rotary_pos_emb(q.view(shape), k.view(shape), cos, sin, unsqueeze_dim=2)
+        return q, k, v.view(shape)
 
 
 def replace_attention(module):

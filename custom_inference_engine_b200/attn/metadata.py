@@ -29,6 +29,9 @@ class AttentionMetadata:
         # (decode: lens[slot_ids] + 1, mixed: lens[slot_ids]) computed once by
         # the caller; when None every layer computes them from the KV storage.
         self.attn_lens = None
+        # Optional, not in the reference: for a mixed pass over 8-bit pages, the
+        # slots' lengths with this pass's rows (attn_lens + chunk lengths).
+        self.read_lens = None
         # Optional, not in the reference: a mixed pass with this set runs its
         # RoPE, K/V write and attention as one call (rope_kv_mixed_attention);
         # left False, the pass keeps the reference's gqa_mixed_attention op,

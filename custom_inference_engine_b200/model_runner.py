@@ -19,6 +19,10 @@ This is the harness that measures Qwen2.5-0.5B-shape tokens/s and checks greedy
 tokens against HF's own attention; ``serving.py`` drives it with a request
 queue (Poisson arrivals, continuous batching). Every admitted slot gets enough
 pages up front for its prompt plus its new tokens.
+
+``PagedRunner(kv_cache_dtype=torch.int8)`` keeps the KV pages in 8 bits, and a
+``Sampling`` replaces the greedy token by a sampled one
+(``inference::sample_rows``).
 """
 from __future__ import annotations
 
@@ -119,6 +123,25 @@ class PrefillResult:
     forward_passes: int
 
 
+@dataclass(frozen=True)
+class Sampling:
+    """How tokens are drawn: ``inference::sample_rows``' temperature (0: greedy), top-k
+    (0: off), top-p (1: off) and min-p (0: off), one value or one per row."""
+    temperature: float = 1.0
+    top_k: int = 0
+    top_p: float = 1.0
+    min_p: float = 0.0
+
+    def columns(self, rows: int, device):
+        """The op's four per-row tensors."""
+        def column(x, dtype):
+            t = torch.as_tensor(x, dtype=dtype, device=device)
+            return t.expand(rows).contiguous() if t.dim() == 0 else t.contiguous()
+
+        return (column(self.temperature, torch.float32), column(self.top_k, torch.int64),
+                column(self.top_p, torch.float32), column(self.min_p, torch.float32))
+
+
 class PagedRunner:
     """Slots, pages and forward passes of one model replica on one GPU.
 
@@ -130,9 +153,9 @@ class PagedRunner:
     def __init__(self, model, max_cache_len: int, n_slots: int, page_seed: int = 0,
                  token_budget: int = 2048, fused_body: bool = True, mixed_graphs: bool = True,
                  block_table_dtype=torch.int64, fused_lm_head: bool = True,
-                 fused_mixed_attention: bool = True):
+                 fused_mixed_attention: bool = True, kv_cache_dtype=None, sample_seed: int = 0):
         from .attn.core import use_cuda_attention
-        from .kv_cache.storage import KVStorage
+        from .kv_cache.storage import KVStorage, QuantizedKVStorage
 
         self.model = model
         use_cuda_attention(model)
@@ -142,8 +165,15 @@ class PagedRunner:
         self.fused_mixed_attention = fused_mixed_attention
         self.device = next(model.parameters()).device
         self.dtype = next(model.parameters()).dtype
-        self.kv = KVStorage(model.config, max_cache_len, PAGE_SIZE, n_slots, self.device,
-                            self.dtype, block_table_dtype=block_table_dtype)
+        # kv_cache_dtype: the model's dtype (None), or torch.int8 for 8-bit pages
+        if kv_cache_dtype not in (None, self.dtype, torch.int8):
+            raise ValueError(f"kv_cache_dtype must be {self.dtype} or torch.int8, "
+                             f"not {kv_cache_dtype}")
+        storage = QuantizedKVStorage if kv_cache_dtype == torch.int8 else KVStorage
+        self.kv = storage(model.config, max_cache_len, PAGE_SIZE, n_slots, self.device,
+                          self.dtype, block_table_dtype=block_table_dtype)
+        # random numbers of sampled tokens that the caller does not give itself
+        self.generator = torch.Generator(device=self.device).manual_seed(sample_seed)
         g = torch.Generator().manual_seed(page_seed)
         self.free_pages = (torch.randperm(self.kv.n_pages - 1, generator=g) + 1).tolist()
         self.token_budget = token_budget
@@ -191,6 +221,9 @@ class PagedRunner:
         # the attention lengths of this pass, once for all layers
         lens = self.kv.lens[metadata.slot_ids]
         metadata.attn_lens = lens + 1 if metadata.full_decode else lens
+        if self.kv.quantized and not metadata.full_decode:
+            cu = metadata.cu_seqlens
+            metadata.read_lens = lens + cu[1:] - cu[:-1]
         if self.body is not None:
             return self.body(input_ids, position_ids, self.kv, metadata)
         out = self.model.model(input_ids=input_ids, position_ids=position_ids,
@@ -267,16 +300,29 @@ class PagedRunner:
             self.host_lens[s] += c
         return logits
 
-    def mixed_step(self, slots, token_chunks) -> list:
+    def sample(self, logits, sampling: Sampling, uniform=None) -> torch.Tensor:
+        """A token per row of fp16 logits; ``uniform`` (rows,) fp32 in [0, 1): the rows'
+        random numbers, drawn from the runner's generator when not given."""
+        rows = logits.shape[0]
+        if uniform is None:
+            uniform = torch.rand(rows, generator=self.generator, device=logits.device)
+        return torch.ops.inference.sample_rows(logits, uniform,
+                                               *sampling.columns(rows, logits.device))
+
+    def mixed_step(self, slots, token_chunks, sampling=None) -> list:
         """One mixed pass: sequence i appends ``token_chunks[i]`` (a decode row is
         a chunk of one token) to slot ``slots[i]``; returns the greedy token after
-        each chunk's last row."""
-        return self.mixed_logits(slots, token_chunks).argmax(-1).tolist()
+        each chunk's last row, or a sampled one with ``sampling``."""
+        logits = self.mixed_logits(slots, token_chunks)
+        if sampling is not None:
+            return self.sample(logits, sampling).tolist()
+        return logits.argmax(-1).tolist()
 
-    def prefill(self, slots, prompts) -> PrefillResult:
+    def prefill(self, slots, prompts, sampling=None) -> PrefillResult:
         """Write every prompt into its slot through mixed passes of at most
         ``token_budget`` tokens (a long prompt spans several passes, continuing
-        from its slot's length); returns the greedy token after each prompt."""
+        from its slot's length); returns the greedy token after each prompt, or a
+        sampled one with ``sampling``."""
         remaining = [list(p) for p in prompts]
         done_logits = [None] * len(slots)
         passes = 0
@@ -298,21 +344,24 @@ class PagedRunner:
                         done_logits[i] = logits[j].float()
                 passes += 1
         last = torch.stack(done_logits)
-        return PrefillResult(first_tokens=last.argmax(-1).tolist(), last_logits=last,
-                             forward_passes=passes)
+        first = last.argmax(-1) if sampling is None else self.sample(last.half(), sampling)
+        return PrefillResult(first_tokens=first.tolist(), last_logits=last, forward_passes=passes)
 
-    def decode_graph(self, slots, first_tokens, capture: bool = True) -> "DecodeGraph":
-        return DecodeGraph(self, slots, first_tokens, capture)
+    def decode_graph(self, slots, first_tokens, capture: bool = True,
+                     sampling=None) -> "DecodeGraph":
+        return DecodeGraph(self, slots, first_tokens, capture, sampling)
 
 
 class DecodeGraph:
     """One greedy decode step for a fixed batch of slots: the tokens of the
     previous step in, the next tokens out (``tokens``, device (B,)), every slot
     one position longer. Captured in a CUDA graph unless ``capture`` is False.
-    ``logits`` holds the step's logits only when the runner's ``fused_lm_head``
-    is off."""
+    With ``sampling`` the tokens are sampled, from the step's random numbers in
+    ``uniform`` (B,). ``logits`` holds the step's logits when they are sampled from
+    or the runner's ``fused_lm_head`` is off."""
 
-    def __init__(self, runner: PagedRunner, slots, first_tokens, capture: bool = True):
+    def __init__(self, runner: PagedRunner, slots, first_tokens, capture: bool = True,
+                 sampling=None):
         from .attn.metadata import AttentionMetadata
 
         self.runner = runner
@@ -325,10 +374,18 @@ class DecodeGraph:
         self.tokens = torch.tensor(first_tokens, dtype=torch.long, device=dev)
         self.logits = None
         self.graph = None
+        self.uniform = None
+        if sampling is not None:
+            self.uniform = torch.zeros(B, device=dev)
+            self.columns = sampling.columns(B, dev)
         if capture:
             # the tokens this warm-up produces are discarded: undo its writes
             saved_lens = runner.kv.lens.clone()
             saved_tokens = self.tokens.clone()
+            if runner.kv.quantized:
+                # a row that is written and taken back may leave an 8-bit page at a
+                # larger scale: warm up on the padding slot
+                self.md.write_slot_ids([0] * B)
             side = torch.cuda.Stream()
             side.wait_stream(torch.cuda.current_stream())
             with torch.cuda.stream(side), torch.inference_mode():
@@ -336,6 +393,7 @@ class DecodeGraph:
             torch.cuda.current_stream().wait_stream(side)
             runner.kv.lens.copy_(saved_lens)
             self.tokens.copy_(saved_tokens)
+            self.md.write_slot_ids(self.slots)
             self.graph = torch.cuda.CUDAGraph()
             with torch.inference_mode(), torch.cuda.graph(self.graph):
                 self._step()
@@ -348,14 +406,25 @@ class DecodeGraph:
         pos = kv.lens[self.md.slot_ids].view(1, -1)
         hidden = self.runner._hidden(ids, pos, self.md)
         lm_head = self.runner.model.lm_head
-        if self.runner.fused_lm_head and lm_head.bias is None:
+        if self.uniform is not None:
+            self.logits = lm_head(hidden[0])
+            self.tokens.copy_(torch.ops.inference.sample_rows(self.logits, self.uniform,
+                                                              *self.columns))
+        elif self.runner.fused_lm_head and lm_head.bias is None:
             self.tokens.copy_(torch.ops.inference.lm_head_argmax(hidden[0], lm_head.weight))
         else:
             self.logits = lm_head(hidden[0])
             self.tokens.copy_(torch.ops.inference.argmax_rows(self.logits))
         kv.decode_advance(self.md.slot_ids)
 
-    def step(self) -> torch.Tensor:
+    def step(self, uniform=None) -> torch.Tensor:
+        """The next tokens; ``uniform``: the random numbers of a sampled step, drawn from
+        the runner's generator when not given."""
+        if self.uniform is not None:
+            if uniform is None:
+                self.uniform.uniform_(generator=self.runner.generator)
+            else:
+                self.uniform.copy_(uniform)
         if self.graph is not None:
             self.graph.replay()
         else:

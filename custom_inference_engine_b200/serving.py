@@ -71,15 +71,16 @@ def poisson_requests(n: int, rate: float, seed: int, vocab: int, median_prompt: 
 
 
 class DecodeBuckets:
-    """One captured greedy decode step per batch bucket of ``runner``."""
+    """One captured decode step per batch bucket of ``runner``: greedy, or sampled with
+    ``sampling`` (one value for all rows)."""
 
-    def __init__(self, runner, max_batch: int, buckets=DECODE_BUCKETS):
+    def __init__(self, runner, max_batch: int, buckets=DECODE_BUCKETS, sampling=None):
         from .model_runner import DecodeGraph
 
         self.runner = runner
         self.sizes = [b for b in buckets if b < max_batch] + [max_batch]
         self.sizes = sorted(set(self.sizes))
-        self.graphs = {b: DecodeGraph(runner, [0] * b, [0] * b, capture=True)
+        self.graphs = {b: DecodeGraph(runner, [0] * b, [0] * b, capture=True, sampling=sampling)
                        for b in self.sizes}
 
     def step(self, slots, tokens) -> list:
@@ -89,6 +90,8 @@ class DecodeBuckets:
         g.md.write_slot_ids(slots)
         g.tokens[:n].copy_(g.tokens.new_tensor(tokens))
         g.tokens[n:].zero_()
+        if g.uniform is not None:
+            g.uniform.uniform_(generator=self.runner.generator)
         g.graph.replay()
         out = g.tokens[:n].tolist()
         for s in slots:
@@ -194,11 +197,13 @@ def summarize(requests, trim: float = 0.05) -> dict:
 
 class RunnerEngine:
     """``serve``'s engine on a ``PagedRunner``: mixed passes and decode steps
-    from CUDA graphs captured per token bucket and per batch bucket."""
+    from CUDA graphs captured per token bucket and per batch bucket; greedy, or
+    sampled with a ``Sampling``."""
 
-    def __init__(self, runner, n_slots: int):
+    def __init__(self, runner, n_slots: int, sampling=None):
         self.runner = runner
-        self.buckets = DecodeBuckets(runner, n_slots - 1)
+        self.sampling = sampling
+        self.buckets = DecodeBuckets(runner, n_slots - 1, sampling=sampling)
         runner.capture_mixed_graphs()
 
     @property
@@ -212,7 +217,7 @@ class RunnerEngine:
         self.runner.release(slot)
 
     def mixed_step(self, slots, chunks):
-        return self.runner.mixed_step(slots, chunks)
+        return self.runner.mixed_step(slots, chunks, self.sampling)
 
     def decode_step(self, slots, tokens):
         return self.buckets.step(slots, tokens)
