@@ -580,7 +580,9 @@ extern "C" {
 
 int cie_decode_q8_default_splits(int batch, int device) {
   int sms = 148;
-  if (device >= 0) {
+  if (device >= 0 && device == cie::current_device()) {
+    sms = cie::sm_count();  // (remembered)
+  } else if (device >= 0) {
     int n = 0;
     if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) == cudaSuccess && n > 0)
       sms = n;

@@ -53,6 +53,13 @@ struct Args {
   int64_t n_pages, n_slots, bt_stride;
 };
 
+// Launched as a programmatic dependent of the preceding kernel: nothing is read or written
+// before that one is done, and the next such kernel may be scheduled meanwhile.
+__device__ __forceinline__ void start_as_dependent() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (threadIdx.x == 0) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 __device__ __forceinline__ void load8(const __half* p, int vec, float (&x)[8]) {
   if (vec) {
     const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
@@ -93,22 +100,23 @@ __device__ __forceinline__ float pow2_up(float s) {
 }
 
 // Sequence of token t of a mixed pass: the first b with cu[b + 1] > t, or -1 when
-// t lies in no sequence.
-__device__ __forceinline__ int find_seq(const Args& a, int64_t t) {
-  int lo = 0, hi = a.batch;  // cu[lo] <= t as far as cu is monotone
+// t lies in no sequence. `cu` is a.cu or a copy of it in shared memory.
+__device__ __forceinline__ int find_seq(const int64_t* cu, int batch, int64_t t) {
+  int lo = 0, hi = batch;  // cu[lo] <= t as far as cu is monotone
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
-    if (a.cu[mid + 1] > t) hi = mid;
+    if (cu[mid + 1] > t) hi = mid;
     else lo = mid + 1;
   }
-  return lo < a.batch && a.cu[lo] <= t ? lo : -1;
+  return lo < batch && cu[lo] <= t ? lo : -1;
 }
 
 // Token t leads the rows that this call writes into one page when it is its
 // sequence's first row or sits on row 0 of the page. Returns how many rows that
 // is (0: t leads none, or must not be written), with the sequence and position.
 template <bool kMixed>
-__device__ __forceinline__ int led_rows(const Args& a, int64_t t, int& b, int64_t& pos) {
+__device__ __forceinline__ int led_rows(const Args& a, const int64_t* cu, int64_t t, int& b,
+                                        int64_t& pos) {
   if (t >= a.tokens) return 0;
   if (!kMixed) {
     b = static_cast<int>(t);
@@ -119,17 +127,17 @@ __device__ __forceinline__ int led_rows(const Args& a, int64_t t, int& b, int64_
     }
     pos = a.lens[slot];
   } else {
-    b = find_seq(a, t);
+    b = find_seq(cu, a.batch, t);
     if (b < 0) return 0;
-    pos = a.kv_lens[b] + t - a.cu[b];
-    if (t != a.cu[b] && (pos & (kPage - 1)) != 0) return 0;
+    pos = a.kv_lens[b] + t - cu[b];
+    if (t != cu[b] && (pos & (kPage - 1)) != 0) return 0;
   }
   if (pos < 0 || pos / kPage >= a.bt_stride) {
     raise_error(CIE_DEVERR_BAD_LENGTH);
     return 0;
   }
   if (!kMixed) return 1;
-  int64_t left = min(a.cu[b + 1], a.tokens) - t;
+  const int64_t left = min(cu[b + 1], a.tokens) - t;
   return static_cast<int>(min(left, static_cast<int64_t>(kPage - (pos & (kPage - 1)))));
 }
 
@@ -153,11 +161,7 @@ __device__ __forceinline__ void write_rows(const Args& a, int64_t t, int b, int6
     raise_error(CIE_DEVERR_BAD_SLOT);
     return;
   }
-  const int64_t page = a.table.at(slot * a.bt_stride + pos / kPage);
-  if (page < 0 || page >= a.n_pages) {
-    raise_error(CIE_DEVERR_BAD_PAGE);
-    return;
-  }
+  const int64_t page = a.table.at(slot * a.bt_stride + pos / kPage);  // on its way
   const int off = static_cast<int>(pos & (kPage - 1));
   const int r = lane >> 3, c = lane & 7;
 
@@ -193,11 +197,15 @@ __device__ __forceinline__ void write_rows(const Args& a, int64_t t, int b, int6
       }
     }
   }
-  if (!finite) raise_error(CIE_DEVERR_NONFINITE);
   const bool skip = superseded<kMixed>(a, b, slot, lane);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  if (page < 0 || page >= a.n_pages) {
+    raise_error(CIE_DEVERR_BAD_PAGE);
+    return;
+  }
   if (skip) return;
+  if (!finite) raise_error(CIE_DEVERR_NONFINITE);
 
   float* sp = a.scales + page * 2 * a.hkv + which * a.hkv + h;
   int8_t* tile = (which ? a.v_cache : a.k_cache) + page * a.page_stride + h * a.head_stride;
@@ -242,75 +250,98 @@ __device__ __forceinline__ void write_rows(const Args& a, int64_t t, int b, int6
   if (lane == 0 && scale != stored) *sp = scale;
 }
 
-// One CTA per `tile` consecutive tokens: warp 0 finds the leading tokens, the
-// warps share out their (leader, K / V, kv head) units, then all threads rotate
-// the tile's q rows.
-constexpr int kMaxTile = 32;
+// The first CTAs take `tile` consecutive tokens each: warp 0 finds the leading ones, then
+// the warps share out their (leader, K / V, kv head) units. With the rotary embedding the
+// CTAs behind them rotate q, a thread per (token, head, chunk pair). What bounds a call is
+// the chain of dependent loads (cu_seqlens -> length, slot -> block table -> scale), so
+// a CTA gets few units and the two kinds of work run side by side.
+constexpr int kTile = 4;
+constexpr int kCuShared = 512;  // cu_seqlens entries that are searched in shared memory
 
 template <bool kRope, bool kMixed>
-__global__ void __launch_bounds__(32 * kWarps) update_kernel(const Args a, int tile) {
+__global__ void __launch_bounds__(32 * kWarps) update_kernel(const Args a, int unit_ctas) {
   __shared__ int s_count;
-  __shared__ int s_n[kMaxTile], s_b[kMaxTile];
-  __shared__ int64_t s_t[kMaxTile], s_pos[kMaxTile];
+  __shared__ int s_n[kTile], s_b[kTile];
+  __shared__ int64_t s_t[kTile], s_pos[kTile];
+  __shared__ int64_t s_cu[kMixed ? kCuShared : 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * tile;
-  if (kMixed && blockIdx.x == 0) {
-    // starts at 0 or later, never falls, ends inside the rows
-    bool bad = threadIdx.x == 0 && (a.cu[0] < 0 || a.cu[a.batch] > a.tokens);
-    for (int i = threadIdx.x; i < a.batch; i += blockDim.x) bad |= a.cu[i + 1] < a.cu[i];
-    if (bad) raise_error(CIE_DEVERR_BAD_SEQLENS);
-  }
-  if (warp == 0) {
-    int b = 0;
-    int64_t pos = 0;
-    const int n = lane < tile ? led_rows<kMixed>(a, t0 + lane, b, pos) : 0;
-    const unsigned int leads = __ballot_sync(0xffffffffu, n > 0);
-    if (n > 0) {
-      const int i = __popc(leads & ((1u << lane) - 1u));
-      s_n[i] = n;
-      s_b[i] = b;
-      s_t[i] = t0 + lane;
-      s_pos[i] = pos;
-    }
-    if (lane == 0) s_count = __popc(leads);
-  }
-  __syncthreads();
-  const int per = 2 * a.hkv;
-  for (int u = warp; u < s_count * per; u += kWarps) {
-    const int i = u / per, w = u % per;
-    write_rows<kRope, kMixed>(a, s_t[i], s_b[i], s_pos[i], s_n[i], w / a.hkv, w % a.hkv, lane);
-  }
-  if (kRope) {
-    // thread = (token, q head, c): chunks c and c + 4 are partners of the rotation
-    const int rows = a.hq * 4;
-    const int64_t end = min(a.tokens - t0, static_cast<int64_t>(tile)) * rows;
-    for (int i = threadIdx.x; i < end; i += blockDim.x) {
-      const int64_t tok = t0 + i / rows;
-      const int head = (i % rows) >> 2, c = i & 3;
-      const __half* src = a.qkv + tok * a.qkv_tok + head * kD + 8 * c;
-      float x1[8], x2[8], c1[8], c2[8], s1[8], s2[8];
-      load8(src, 1, x1);
-      load8(src + 32, 1, x2);
-      load8(a.cos + tok * a.cs_tok + 8 * c, 1, c1);
-      load8(a.cos + tok * a.cs_tok + 32 + 8 * c, 1, c2);
-      load8(a.sin + tok * a.cs_tok + 8 * c, 1, s1);
-      load8(a.sin + tok * a.cs_tok + 32 + 8 * c, 1, s2);
-      uint4 lo, hi;
-      __half2* l = reinterpret_cast<__half2*>(&lo);
-      __half2* g = reinterpret_cast<__half2*>(&hi);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int k = 2 * e;
-        l[e] = __floats2half2_rn(rot1(x1[k], -x2[k], c1[k], s1[k]),
-                                 rot1(x1[k + 1], -x2[k + 1], c1[k + 1], s1[k + 1]));
-        g[e] = __floats2half2_rn(rot1(x2[k], x1[k], c2[k], s2[k]),
-                                 rot1(x2[k + 1], x1[k + 1], c2[k + 1], s2[k + 1]));
+  start_as_dependent();
+  if (!kRope || static_cast<int>(blockIdx.x) < unit_ctas) {
+    const int64_t t0 = static_cast<int64_t>(blockIdx.x) * kTile;
+    const int per = 2 * a.hkv;
+    if (!kMixed) {  // every token leads a page of its own
+      for (int u = warp; u < kTile * per; u += kWarps) {
+        const int w = u % per;
+        int b = 0;
+        int64_t pos = 0;
+        if (led_rows<false>(a, nullptr, t0 + u / per, b, pos))
+          write_rows<kRope, false>(a, t0 + u / per, b, pos, 1, w / a.hkv, w % a.hkv, lane);
       }
-      __half* dst = a.q_out + (tok * a.hq + head) * kD + 8 * c;
-      *reinterpret_cast<uint4*>(dst) = lo;
-      *reinterpret_cast<uint4*>(dst + 32) = hi;
+      return;
     }
+    const int64_t* cu = a.cu;
+    {
+      if (blockIdx.x == 0) {
+        // starts at 0 or later, never falls, ends inside the rows
+        bool bad = threadIdx.x == 0 && (a.cu[0] < 0 || a.cu[a.batch] > a.tokens);
+        for (int i = threadIdx.x; i < a.batch; i += blockDim.x) bad |= a.cu[i + 1] < a.cu[i];
+        if (bad) raise_error(CIE_DEVERR_BAD_SEQLENS);
+      }
+      if (a.batch < kCuShared) {
+        for (int i = threadIdx.x; i <= a.batch; i += blockDim.x) s_cu[i] = a.cu[i];
+        cu = s_cu;
+        __syncthreads();
+      }
+    }
+    if (warp == 0) {
+      int b = 0;
+      int64_t pos = 0;
+      const int n = lane < kTile ? led_rows<kMixed>(a, cu, t0 + lane, b, pos) : 0;
+      const unsigned int leads = __ballot_sync(0xffffffffu, n > 0);
+      if (n > 0) {
+        const int i = __popc(leads & ((1u << lane) - 1u));
+        s_n[i] = n;
+        s_b[i] = b;
+        s_t[i] = t0 + lane;
+        s_pos[i] = pos;
+      }
+      if (lane == 0) s_count = __popc(leads);
+    }
+    __syncthreads();
+    for (int u = warp; u < s_count * per; u += kWarps) {
+      const int i = u / per, w = u % per;
+      write_rows<kRope, kMixed>(a, s_t[i], s_b[i], s_pos[i], s_n[i], w / a.hkv, w % a.hkv, lane);
+    }
+    return;
   }
+  // chunks c and c + 4 of a head are partners of the rotation
+  const int64_t i = static_cast<int64_t>(blockIdx.x - unit_ctas) * blockDim.x + threadIdx.x;
+  const int rows = a.hq * 4;
+  const int64_t tok = i / rows;
+  if (tok >= a.tokens) return;
+  const int head = static_cast<int>(i - tok * rows) >> 2, c = static_cast<int>(i) & 3;
+  const __half* src = a.qkv + tok * a.qkv_tok + head * kD + 8 * c;
+  float x1[8], x2[8], c1[8], c2[8], s1[8], s2[8];
+  load8(src, 1, x1);
+  load8(src + 32, 1, x2);
+  load8(a.cos + tok * a.cs_tok + 8 * c, 1, c1);
+  load8(a.cos + tok * a.cs_tok + 32 + 8 * c, 1, c2);
+  load8(a.sin + tok * a.cs_tok + 8 * c, 1, s1);
+  load8(a.sin + tok * a.cs_tok + 32 + 8 * c, 1, s2);
+  uint4 lo, hi;
+  __half2* l = reinterpret_cast<__half2*>(&lo);
+  __half2* g = reinterpret_cast<__half2*>(&hi);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int k = 2 * e;
+    l[e] = __floats2half2_rn(rot1(x1[k], -x2[k], c1[k], s1[k]),
+                             rot1(x1[k + 1], -x2[k + 1], c1[k + 1], s1[k + 1]));
+    g[e] = __floats2half2_rn(rot1(x2[k], x1[k], c2[k], s2[k]),
+                             rot1(x2[k + 1], x1[k + 1], c2[k + 1], s2[k + 1]));
+  }
+  __half* dst = a.q_out + (tok * a.hq + head) * kD + 8 * c;
+  *reinterpret_cast<uint4*>(dst) = lo;
+  *reinterpret_cast<uint4*>(dst + 32) = hi;
 }
 
 // ---- read back -------------------------------------------------------------------
@@ -330,56 +361,105 @@ struct ReadArgs {
   int64_t page_stride, head_stride, out_page, out_head;
 };
 
-// 16 codes -> 16 fp16 values code * scale (one rounding; exact for power-of-two scales)
-__device__ __forceinline__ void dequant16(uint4 codes, float scale, uint4& lo, uint4& hi) {
-  const signed char* c = reinterpret_cast<const signed char*>(&codes);
-  __half2* l = reinterpret_cast<__half2*>(&lo);
-  __half2* h = reinterpret_cast<__half2*>(&hi);
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    l[e] = __floats2half2_rn(c[2 * e] * scale, c[2 * e + 1] * scale);
-    h[e] = __floats2half2_rn(c[8 + 2 * e] * scale, c[8 + 2 * e + 1] * scale);
-  }
+// Two biased codes (code + 128) of `w`, picked by the selector, as fp16 numbers: 0x64 over a
+// byte u is 1024 + u, and subtracting 1152 is exact.
+__device__ __forceinline__ __half2 two_codes(uint32_t w, uint32_t sel) {
+  const uint32_t h = __byte_perm(w, 0x64646464u, sel);
+  return __hsub2(*reinterpret_cast<const __half2*>(&h), __floats2half2_rn(1152.f, 1152.f));
 }
 
-// Grid (x, sequence): thread = 16 codes of a page; a sequence's pages are dealt to
-// its CTAs one by one.
+// 8 codes -> 8 fp16 values code * scale, rounded once (exact for the powers of two that
+// the update calls store): in fp16 when the scale is a fp16 number, else in fp32.
+__device__ __forceinline__ uint4 dequant8(uint2 codes, float scale) {
+  const uint32_t w[2] = {codes.x ^ 0x80808080u, codes.y ^ 0x80808080u};
+  const __half s = __float2half_rn(scale);
+  const bool exact = __half2float(s) == scale;
+  const __half2 s2 = __half2half2(s);
+  uint4 r;
+  __half2* o = reinterpret_cast<__half2*>(&r);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const __half2 c = two_codes(w[e >> 1], e & 1 ? 0x4342 : 0x4140);
+    if (exact) {
+      o[e] = __hmul2_rn(c, s2);
+    } else {
+      const float2 f = __half22float2(c);
+      o[e] = __floats2half2_rn(f.x * scale, f.y * scale);
+    }
+  }
+  return r;
+}
+
+// Grid (x, sequence): a warp per K or V of a page, a lane per 8 codes (256-byte reads,
+// 512-byte writes), two heads' reads in flight before their first write; a sequence's
+// pages are dealt to its warps one by one. Bound by bandwidth, 1 byte read and 2 written
+// a value.
 __global__ void __launch_bounds__(256) read_kernel(const ReadArgs a) {
-  const int b = blockIdx.y;
+  const int b = blockIdx.y, lane = threadIdx.x & 31;
+  start_as_dependent();
   const int64_t slot = a.slot_ids[b];
+  int64_t len = a.lens[b], start = a.starts ? a.starts[b] : 0;
   if (slot < 0 || slot >= a.n_slots) {
     if (blockIdx.x == 0 && threadIdx.x == 0) raise_error(CIE_DEVERR_BAD_SLOT);
     return;
   }
-  int64_t len = a.lens[b];
   if (len > a.bt_stride * kPage) {
     if (blockIdx.x == 0 && threadIdx.x == 0) raise_error(CIE_DEVERR_BAD_LENGTH);
     len = a.bt_stride * kPage;
   }
-  int64_t start = a.starts ? a.starts[b] : 0;
   if (start < 0) start = 0;
-  const int items = 2 * a.hkv * kPage * 4;  // 16-code chunks of one page
+  const int which = (threadIdx.x >> 5) & 1;
+  const int8_t* pool = which ? a.v : a.k;
+  __half* out = which ? a.v_out : a.k_out;
   const int64_t pages = (len + kPage - 1) / kPage;
-  for (int64_t j = start / kPage + blockIdx.x; j < pages; j += gridDim.x) {
-    const int64_t page = a.table.at(slot * a.bt_stride + j);
+  const int64_t* wide = static_cast<const int64_t*>(a.table.ptr);
+  const int32_t* narrow = static_cast<const int32_t*>(a.table.ptr);
+  const int64_t row = slot * a.bt_stride;
+  auto entry = [&](int64_t j) -> int64_t {
+    return j < pages ? (a.table.wide ? wide[row + j] : narrow[row + j]) : 0;
+  };
+  int64_t j = start / kPage + static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  int64_t page = entry(j);
+#pragma unroll 1
+  for (; j < pages;) {
+    const int64_t next = j + static_cast<int64_t>(gridDim.x) * 4;
+    const int64_t next_page = entry(next);
     if (page < 0 || page >= a.n_pages) {
-      if (threadIdx.x == 0) raise_error(CIE_DEVERR_BAD_PAGE);
-      continue;
+      if (lane == 0) raise_error(CIE_DEVERR_BAD_PAGE);
+    } else {
+      const float* scales = a.scales + (page * 2 + which) * a.hkv;
+      const int8_t* src = pool + page * a.page_stride + lane * 8;
+      __half* dst = out + page * a.out_page + lane * 8;
+      // rows lo .. hi - 1 of the page; chunk e of this lane is in row 4 e + lane / 8
+      const int lo = static_cast<int>(max(start - j * kPage, int64_t(0))) - (lane >> 3);
+      const int hi = static_cast<int>(min(len - j * kPage, int64_t(kPage))) - (lane >> 3);
+#pragma unroll 1
+      for (int h = 0; h < a.hkv; h += 2) {
+        uint2 u[2][4];
+        float s[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          if (h + k < a.hkv) {
+            s[k] = scales[h + k];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              u[k][e] = *reinterpret_cast<const uint2*>(src + (h + k) * a.head_stride + 256 * e);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          if (h + k < a.hkv) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (4 * e >= lo && 4 * e < hi)
+                *reinterpret_cast<uint4*>(dst + (h + k) * a.out_head + 256 * e) =
+                    dequant8(u[k][e], s[k]);
+          }
+        }
+      }
     }
-    for (int i = threadIdx.x; i < items; i += blockDim.x) {
-      const int c = i & 3, row = (i >> 2) & (kPage - 1);
-      const int wh = i >> 6, which = wh / a.hkv, h = wh % a.hkv;
-      const int64_t pos = j * kPage + row;
-      if (pos < start || pos >= len) continue;
-      const int8_t* src = (which ? a.v : a.k) + page * a.page_stride + h * a.head_stride;
-      __half* dst = (which ? a.v_out : a.k_out) + page * a.out_page + h * a.out_head;
-      const float scale = a.scales[page * 2 * a.hkv + wh];
-      uint4 lo, hi;
-      dequant16(*reinterpret_cast<const uint4*>(src + row * kD + 16 * c), scale, lo, hi);
-      uint4* d = reinterpret_cast<uint4*>(dst + row * kD + 16 * c);
-      d[0] = lo;
-      d[1] = hi;
-    }
+    j = next;
+    page = next_page;
   }
 }
 
@@ -404,18 +484,30 @@ int check_pool(const void* k, const void* v, const void* scales, int hkv, int he
   return CIE_OK;
 }
 
+// Launch as a programmatic dependent (start_as_dependent).
+template <typename Kernel, typename... Params>
+int launch(const char* what, Kernel kernel, dim3 grid, cie_stream_t stream, Params... params) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(32 * kWarps);
+  cfg.stream = reinterpret_cast<cudaStream_t>(stream);
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, params...);
+  if (e != cudaSuccess) return fail(CIE_ERR_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
+  return CIE_OK;
+}
+
 template <bool kRope, bool kMixed>
 int launch_update(const Args& a, cie_stream_t stream) {
-  // decode: every token leads its own page; mixed: a sequence's chunk has one
-  // leader per page, so a CTA takes a page's worth of tokens
-  const int tile = kMixed ? 16 : 2;
-  const int64_t grid = (a.tokens + tile - 1) / tile;
-  if (grid > 0x7fffffff) return fail(CIE_ERR_OVERFLOW, "too many tokens");
-  update_kernel<kRope, kMixed><<<static_cast<unsigned>(grid), 32 * kWarps, 0,
-                                 reinterpret_cast<cudaStream_t>(stream)>>>(a, tile);
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return fail(CIE_ERR_CUDA, "kv_q8 update launch: %s", cudaGetErrorString(e));
-  return CIE_OK;
+  const int64_t units = (a.tokens + kTile - 1) / kTile;
+  const int64_t rotate = kRope ? (a.tokens * a.hq * 4 + 32 * kWarps - 1) / (32 * kWarps) : 0;
+  if (units + rotate > 0x7fffffff) return fail(CIE_ERR_OVERFLOW, "too many tokens");
+  return launch("kv_q8 update", update_kernel<kRope, kMixed>,
+                dim3(static_cast<unsigned>(units + rotate)), stream, a, static_cast<int>(units));
 }
 
 // Checks and launch of every update entry point: mixed when a.cu is set, with the
@@ -458,15 +550,11 @@ int read(const ReadArgs& a, int batch, int head_dim, int page_size, cie_stream_t
     return fail(CIE_ERR_INVALID_ARGUMENT, "overlapping output strides");
   if ((a.out_page % 8) || (a.out_head % 8) || !aligned16(a.k_out) || !aligned16(a.v_out))
     return fail(CIE_ERR_ALIGNMENT, "outputs must be 16-byte aligned with 16-byte strides");
-  // lengths are on the device: as many CTAs as the SMs hold, at most one per page
-  // of the block-table row
+  // lengths are on the device: as many CTAs as the SMs hold, at most one per four pages of
+  // the block-table row
   int64_t per = (8LL * sm_count() + batch - 1) / batch;
-  if (per > a.bt_stride) per = a.bt_stride;
-  read_kernel<<<dim3(static_cast<unsigned>(per), batch), 256, 0,
-                reinterpret_cast<cudaStream_t>(stream)>>>(a);
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return fail(CIE_ERR_CUDA, "kv_q8 read launch: %s", cudaGetErrorString(e));
-  return CIE_OK;
+  if (per > (a.bt_stride + 3) / 4) per = (a.bt_stride + 3) / 4;
+  return launch("kv_q8 read", read_kernel, dim3(static_cast<unsigned>(per), batch), stream, a);
 }
 
 Args pool_args(void* k_cache, void* v_cache, float* scales, const int64_t* slot_ids,

@@ -411,10 +411,13 @@ cie_stream_t current_stream() {
 // Every tensor on the first one's device: a pointer of another device must not
 // reach a kernel. (Messages hold text only: formatting a number into a TORCH_CHECK
 // message ends the process in an extension built against this torch.)
-void check_same_device(const at::Tensor& first, std::initializer_list<at::Tensor> others) {
-  for (const at::Tensor& t : others)
+template <typename... Tensors>
+void check_same_device(const at::Tensor& first, const Tensors&... others) {
+  auto check = [&](const at::Tensor& t) {
     TORCH_CHECK(t.device() == first.device(), "all tensors must be on ", first.device().str(),
                 ", got ", t.device().str());
+  };
+  (check(others), ...);
 }
 
 void check_q8_pool(const at::Tensor& k, const at::Tensor& v, const at::Tensor& scales) {
@@ -426,7 +429,7 @@ void check_q8_pool(const at::Tensor& k, const at::Tensor& v, const at::Tensor& s
   TORCH_CHECK(scales.scalar_type() == at::kFloat && scales.is_contiguous() && scales.dim() == 3 &&
                   scales.size(0) == k.size(0) && scales.size(1) == 2 && scales.size(2) == k.size(1),
               "kv_scales must be a contiguous float32 (n_pages, 2, H_kv) tensor");
-  check_same_device(k, {v, scales});
+  check_same_device(k, v, scales);
 }
 
 void check_q8_tables(const at::Tensor& k, const at::Tensor& slot_ids,
@@ -437,14 +440,14 @@ void check_q8_tables(const at::Tensor& k, const at::Tensor& slot_ids,
   TORCH_CHECK(block_table.dim() == 2 && block_table.size(1) == k.size(0) &&
                   block_table.stride(1) == 1,
               "block_table must be (n_slots, n_pages) with contiguous rows");
-  check_same_device(k, {slot_ids, block_table});
+  check_same_device(k, slot_ids, block_table);
 }
 
 void check_per_sequence(const at::Tensor& t, const at::Tensor& k, int64_t n, const char* name) {
   check_i64(t, name);
   TORCH_CHECK(t.dim() == 1 && t.size(0) == n && t.is_contiguous(), name,
               " must be contiguous 1-D with ", std::to_string(n), " values");
-  check_same_device(k, {t});
+  check_same_device(k, t);
 }
 
 void check_q8_rows(const at::Tensor& k, const at::Tensor& k_new, const at::Tensor& v_new) {
@@ -454,7 +457,7 @@ void check_q8_rows(const at::Tensor& k, const at::Tensor& k_new, const at::Tenso
                   k_new.size(3) == k.size(3) && k_new.sizes() == v_new.sizes(),
               "new rows must be (1, T, H_kv, D)");
   TORCH_CHECK(k_new.stride(3) == 1 && v_new.stride(3) == 1, "new rows need unit inner stride");
-  check_same_device(k, {k_new, v_new});
+  check_same_device(k, k_new, v_new);
 }
 
 void check_q8_rope(const at::Tensor& qkv, const at::Tensor& cos, const at::Tensor& sin,
@@ -471,7 +474,7 @@ void check_q8_rope(const at::Tensor& qkv, const at::Tensor& cos, const at::Tenso
                   cos.size(0) == 1 && cos.size(1) == qkv.size(1) && cos.size(2) == k.size(3) &&
                   cos.stride(2) == 1,
               "cos / sin must be (1, T, D) with unit inner stride");
-  check_same_device(k, {qkv, cos, sin});
+  check_same_device(k, qkv, cos, sin);
 }
 
 // Slots that both the lengths (per slot) and the block table have.
@@ -482,7 +485,7 @@ int64_t slots_of(const at::Tensor& lens, const at::Tensor& block_table) {
 void check_slot_lens(const at::Tensor& lens, const at::Tensor& k) {
   check_i64(lens, "lens");
   TORCH_CHECK(lens.dim() == 1 && lens.is_contiguous(), "lens (per slot) must be contiguous 1-D");
-  check_same_device(k, {lens});
+  check_same_device(k, lens);
 }
 
 void kv_q8_decode_update(at::Tensor& k_cache, at::Tensor& v_cache, at::Tensor& kv_scales,
@@ -611,7 +614,7 @@ void kv_q8_read(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::
                   k_out.strides() == v_out.strides() && k_out.stride(3) == 1 &&
                   k_out.stride(2) == k_out.size(3),
               "k_out / v_out must have the cache's shape, equal strides and dense rows");
-  check_same_device(k_cache, {k_out, v_out});
+  check_same_device(k_cache, k_out, v_out);
   c10::cuda::CUDAGuard guard(k_cache.device());
   const int st = with_table(
       block_table,
@@ -640,7 +643,7 @@ at::Tensor gqa_decode_attention_q8(const at::Tensor& q, const at::Tensor& k, con
               "q must be a contiguous float16 (1, B, H_q, D) tensor");
   TORCH_CHECK(k.size(1) > 0 && q.size(2) % k.size(1) == 0 && q.size(3) == k.size(3),
               "H_q must be a multiple of H_kv and head_dim the cache's");
-  check_same_device(k, {q});
+  check_same_device(k, q);
   c10::cuda::CUDAGuard guard(q.device());
   at::Tensor o = at::empty_like(q);
   if (B == 0) return o;
@@ -784,7 +787,7 @@ at::Tensor sample_rows(const at::Tensor& logits, const at::Tensor& uniform,
   auto per_row = [&](const at::Tensor& t, at::ScalarType type, const char* name) {
     TORCH_CHECK(t.scalar_type() == type && t.is_contiguous() && t.numel() == rows, name,
                 " must be a contiguous ", c10::toString(type), " tensor with one value per row");
-    check_same_device(logits, {t});
+    check_same_device(logits, t);
   };
   per_row(uniform, at::kFloat, "uniform");
   per_row(temperature, at::kFloat, "temperature");
