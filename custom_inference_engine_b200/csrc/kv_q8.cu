@@ -518,7 +518,8 @@ int update(Args a, bool rope, bool mixed, int head_dim, int page_size, cie_strea
   const int st = check_pool(a.k_cache, a.v_cache, a.scales, a.hkv, head_dim, page_size, a.n_pages,
                             a.n_slots, a.bt_stride, a.page_stride, a.head_stride);
   if (st != CIE_OK) return st;
-  if (!a.slot_ids || !a.table.ptr || (mixed ? !a.cu || !a.kv_lens : !a.lens))
+  if ((mixed && !a.cu) ||
+      (a.batch > 0 && (!a.slot_ids || !a.table.ptr || (mixed ? !a.kv_lens : !a.lens))))
     return fail(CIE_ERR_INVALID_ARGUMENT, "null lengths / slot_ids / block_table");
   if (rope) {
     if (!a.qkv || !a.cos || !a.sin || !a.q_out)

@@ -29,7 +29,10 @@
  * page was written at once. code * scale is exact in fp16. Rows a call does
  * not write, and their codes, stay as they were unless the scale grew.
  * Values beyond +-65024 saturate; an infinity is stored saturated and a NaN as
- * 0, and both set CIE_DEVERR_NONFINITE.
+ * 0, and both set CIE_DEVERR_NONFINITE. Pages may be shared by slots that read
+ * them; the sequences of one update call must write different pages.
+ * The kernels are programmatic dependents of the preceding kernel in `stream` and
+ * touch nothing before it is done.
  */
 #ifndef CIE_KV_Q8_H_
 #define CIE_KV_Q8_H_

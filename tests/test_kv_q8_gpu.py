@@ -434,6 +434,46 @@ def test_captured_replayed_and_on_a_side_stream(ops, cuda_device):
             assert torch.equal(a, b)
 
 
+def test_a_pass_without_sequences_rotates_its_rows(ops, cuda_device):
+    dev = cuda_device
+    (k, v, s, bt), g = _pool([20], 2, 3, dev)
+    x = _rows(5, 14, 2, g, dev)
+    cos, sin = _rotary(torch.arange(5), dev)
+    none = torch.zeros(0, dtype=torch.long, device=dev)
+    before = [t.clone() for t in (k, v, s)]
+    q = ops.rope_kv_q8_mixed_update(x.reshape(1, 5, -1), cos, sin, k, v, s,
+                                    torch.zeros(1, dtype=torch.long, device=dev), none, none, bt)
+    assert torch.equal(q.cpu(), ref.rope_fp32(x[:, :, :14].cpu(), cos.cpu(), sin.cpu()).half())
+    for a, b in zip((k, v, s), before):
+        assert torch.equal(a, b)
+
+
+def test_pools_beyond_32_bit_offsets(ops, cuda_device):
+    """The last pages of pools of more than 2^31 bytes (and 2^31 fp16 values read back)."""
+    dev, n_pages, n = cuda_device, 1_100_000, 200
+    k, v = (torch.zeros(n_pages, 2, PAGE, D, dtype=torch.int8, device=dev) for _ in range(2))
+    s = torch.zeros(n_pages, 2, 2, device=dev)
+    out = [torch.zeros(k.shape, dtype=torch.half, device=dev) for _ in range(2)]
+    used = -(-n // PAGE)
+    bt = torch.zeros(2, n_pages, dtype=torch.int32, device=dev)
+    bt[1, :used] = torch.arange(n_pages - used, n_pages, dtype=torch.int32, device=dev)
+    g = torch.Generator().manual_seed(1)
+    rows = torch.randn(2, 1, n, 2, D, generator=g).half()
+    t = lambda *x: torch.tensor(x, device=dev)
+    ops.kv_q8_mixed_update(k, v, s, t(0, n), t(0), t(1), bt, rows[0].to(dev), rows[1].to(dev))
+    small = [torch.zeros(used, 2, PAGE, D, dtype=torch.int8) for _ in range(2)]
+    scales = torch.zeros(used, 2, 2)
+    near = torch.stack([torch.zeros(used), torch.arange(used)]).long()
+    ref.update(*small, scales, [(1, 0, 0, n)], near, rows[0, 0], rows[1, 0])
+    assert torch.equal(k[-used:].cpu(), small[0]) and torch.equal(v[-used:].cpu(), small[1])
+    assert torch.equal(s[-used:].cpu(), scales) and not k[:1000].any()
+    ops.kv_q8_read(k, v, s, None, t(n), t(1), bt, *out)
+    back = (small[0].float() * scales[:, 0, :, None, None]).half()
+    assert torch.equal(out[0][n_pages - used:-1].cpu(), back[:-1]) and not out[0][:1000].any()
+    args = (torch.randn(1, 1, 14, D, generator=g).half().to(dev), k, v, s, t(n), t(1), bt)
+    _near(ops.gqa_decode_attention_q8(*args), args)
+
+
 def test_op_refusals(ops, cuda_device):
     dev = cuda_device
     q, k, v, s, lens, slots, bt = _attend(dev, [20, 40], 2, 7, 1)

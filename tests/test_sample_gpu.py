@@ -153,6 +153,32 @@ def test_rows_at_any_alignment_and_stride(ops, cuda_device):
     assert cabi.sample_rows(buf, u.to(dev), t.to(dev)).tolist() == _want(buf, u, t)
 
 
+def test_a_row_alone_and_rows_that_coincide(ops, cuda_device):
+    dev = cuda_device
+    x, g = _logits(1, 4000, 19, dev)
+    u, t = torch.rand(1, generator=g).to(dev), torch.ones(1, device=dev)
+    got = ops.sample_rows(x[0], u, t)
+    assert got.shape == () and [got.item()] == _want(x, u.cpu(), t.cpu())
+    with pytest.raises(RuntimeError):  # rows may not overlap
+        ops.sample_rows(x.expand(3, 4000), u.repeat(3), t.repeat(3))
+
+
+def test_constant_rows(ops, cuda_device):
+    """Every token the same: the counters hold a whole part of a row, and the cumulative
+    mass meets its random number exactly."""
+    dev = cuda_device
+    for vocab in (4, 65528, 131056, 262144, 524224):
+        x = torch.full((5, vocab), 3.25, device=dev).half()
+        u = torch.tensor([0.0, 0.25, 0.5, 0.75, 1 - 2.0 ** -24])
+        t = torch.full((5,), 0.7, device=dev)
+        got = ops.sample_rows(x, u.to(dev), t)
+        assert got.tolist() == [min(int(a * vocab), vocab - 1) for a in u.tolist()], vocab
+        k = torch.full((5,), vocab // 2, device=dev)
+        got = ops.sample_rows(x, u.to(dev), t, k, top_p=torch.full((5,), 0.5, device=dev))
+        n = vocab // 4
+        assert got.tolist() == [min(int(a * n), n - 1) for a in u.tolist()], vocab
+
+
 def test_follows_the_distribution(ops, cuda_device):
     """Evenly spaced numbers over one row: the tokens' counts are their probabilities
     to within one."""
