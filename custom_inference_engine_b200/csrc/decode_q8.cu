@@ -225,28 +225,28 @@ __global__ void __launch_bounds__(32 * kWarps, 2) decode_q8_split_kernel(const P
   float acc[kHeads][4][4];
 
   {
-          // Q^T as the B operand: lane (g, t) holds query head g, dims 16 t .. 16 t + 15
-          const bool valid = g < p.group;
-    #pragma unroll
-          for (int u = 0; u < kHeads; ++u) {
-            const uint4* qr = reinterpret_cast<const uint4*>(
-                p.q + (static_cast<int64_t>(b) * H_Q + (h0 + u) * p.group + (valid ? g : 0)) * kD +
-                16 * t4);
-            const uint4 a = valid ? qr[0] : make_uint4(0, 0, 0, 0);
-            const uint4 d = valid ? qr[1] : make_uint4(0, 0, 0, 0);
-            bq[u][0][0] = a.x;
-            bq[u][0][1] = a.y;
-            bq[u][1][0] = a.z;
-            bq[u][1][1] = a.w;
-            bq[u][2][0] = d.x;
-            bq[u][2][1] = d.y;
-            bq[u][3][0] = d.z;
-            bq[u][3][1] = d.w;
-            m[u][0] = m[u][1] = -CUDART_INF_F;
-            l[u][0] = l[u][1] = 0.f;
-    #pragma unroll
-            for (int e = 0; e < 16; ++e) acc[u][e >> 2][e & 3] = 0.f;
-          }
+    // Q^T as the B operand: lane (g, t) holds query head g, dims 16 t .. 16 t + 15
+    const bool valid = g < p.group;
+#pragma unroll
+    for (int u = 0; u < kHeads; ++u) {
+      const uint4* qr = reinterpret_cast<const uint4*>(
+          p.q + (static_cast<int64_t>(b) * H_Q + (h0 + u) * p.group + (valid ? g : 0)) * kD +
+          16 * t4);
+      const uint4 a = valid ? qr[0] : make_uint4(0, 0, 0, 0);
+      const uint4 d = valid ? qr[1] : make_uint4(0, 0, 0, 0);
+      bq[u][0][0] = a.x;
+      bq[u][0][1] = a.y;
+      bq[u][1][0] = a.z;
+      bq[u][1][1] = a.w;
+      bq[u][2][0] = d.x;
+      bq[u][2][1] = d.y;
+      bq[u][3][0] = d.z;
+      bq[u][3][1] = d.w;
+      m[u][0] = m[u][1] = -CUDART_INF_F;
+      l[u][0] = l[u][1] = 0.f;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[u][e >> 2][e & 3] = 0.f;
+    }
   }
   uint32_t high;
   asm volatile("mov.u32 %0, %%laneid;" : "=r"(high));
@@ -444,9 +444,11 @@ __global__ void __launch_bounds__(kFold > 1 ? 32 * kFold : 1024) merge_q8_kernel
   // (the split kernel does not write slots and lengths)
   const int n = seq_pages(p, b);
   const int pps = decode::split_pages(n, p.num_splits);
+  // Every CTA waits, also one with nothing to merge: a grid that ended without waiting
+  // would let the kernel after it start while the split kernel still writes its rows.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (n <= pps) return;
   const int splits = (n + pps - 1) / pps;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   float M = -CUDART_INF_F, l = 0.f;
   float2 acc = make_float2(0.f, 0.f);
 #pragma unroll 4
