@@ -8,7 +8,8 @@ The package mirrors the reference engine's attention boundary:
   ``TritonQwen2Attention`` / ``use_triton_attention``;
 * ``custom_inference_engine_b200.attn.metadata`` -- ``AttentionMetadata``;
 * ``custom_inference_engine_b200.kv_cache.storage`` -- ``KVStorage`` whose
-  ``decode_update`` / ``mixed_update`` run the CUDA KV-page scatter.
+  ``decode_update`` / ``mixed_update`` run the CUDA KV-page scatter, and
+  ``QuantizedKVStorage`` with 8-bit pages.
 
 All compute runs in hand-written CUDA kernels inside ``libcie_attention.so``
 (C ABI, declared in ``include/cie_attention.h``); ``_cie_torch_ops.so``
