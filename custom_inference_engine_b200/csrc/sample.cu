@@ -12,11 +12,12 @@
 // One cluster of C CTAs per row, C parts of the row:
 //   1. every CTA counts its part into 2^16 16-bit counters in its shared memory
 //      (two to a word, 128 KiB; a part has at most 65528 tokens, so none overflows);
-//   2. the keys form 256 chunks of 256; warps sum a chunk's counters over the
-//      cluster (distributed shared memory) and hand CTA 0 the chunk's tokens,
-//      mass and tokens that min-p keeps;
+//   2. the keys form 256 chunks of 8 entries of 32 keys (an entry lies in one binade, so its
+//      weights are a geometric sequence); warps sum the counters over the cluster
+//      (distributed shared memory) and hand CTA 0 each chunk's tokens, mass and tokens
+//      that min-p keeps, and each entry's weight and what comes before it in its chunk;
 //   3. CTA 0's first warp finds the kept prefix and the key of the sampled token
-//      with its rank among the tokens of that key, descending into one chunk for
+//      with its rank among the tokens of that key, descending to one entry's keys for
 //      each prefix;
 //   4. the CTA whose part holds that token looks it up in the row.
 #include <cooperative_groups.h>
@@ -34,7 +35,9 @@ namespace cg = cooperative_groups;
 
 constexpr int kThreads = 512;
 constexpr int kKeys = 1 << 16;
-constexpr int kChunks = 256;              // of 256 keys, 8 per lane
+constexpr int kChunks = 256;              // of 8 entries
+constexpr int kEntries = 8 * kChunks;     // of 32 keys
+constexpr int kUnroll = 4;                // 16-byte units of the row in flight per thread
 constexpr int kMaxPart = 65528;           // tokens of a part: multiple of 8 below 2^16
 constexpr int kMaxCluster = 8;
 // keys of some values
@@ -54,14 +57,30 @@ struct Params {
   int part;                 // tokens per CTA, multiple of 8
 };
 
+// Powers 1, 2, 4, 8 and 16 of the weight of a key by that of the one before.
+struct Ratios {
+  double r1, r2, r4, r8, r16;
+
+  __device__ __forceinline__ double power(int n) const {  // 0 <= n < 32
+    const double a = (n & 1 ? r1 : 1.0) * (n & 2 ? r2 : 1.0);
+    const double b = (n & 4 ? r4 : 1.0) * (n & 8 ? r8 : 1.0);
+    return n & 16 ? a * (b * r16) : a * b;
+  }
+};
+
 struct alignas(16) Shared {
   uint32_t hist[kKeys / 2];       // counter of key d: half d & 1 of word d >> 1
-  // CTA 0, per chunk: mass and tokens, those of all chunks before, and those that min-p
+  Ratios ratios[32];              // of each binade
+  // CTA 0, per entry: weight of its first key (at or behind the row's largest logit), and
+  // mass and tokens of the entries before it in its chunk
+  double entry_base[kEntries], entry_mass[kEntries];
+  // per chunk: mass and tokens, those of all chunks before, and those that min-p
   // keeps (`some` says that it drops any)
   double mass[kChunks], mass_before[kChunks], mass_above[kChunks];
+  int entry_count[kEntries];
   int count[kChunks], before[kChunks], above[kChunks];
   int some;
-  int warp_sum[kThreads / 32];
+  alignas(8) int hits[2][kUnroll * kThreads / 32];
   unsigned int top, bottom;       // smallest and largest key of this CTA's part
   unsigned int tops[kMaxCluster], bottoms[kMaxCluster];  // and of every part
   unsigned int key;               // the sampled token's key and its rank among this
@@ -91,13 +110,16 @@ __device__ __forceinline__ double as_double(unsigned int c) {
 
 // fp16 value of a finite key, and the step (< 0) to the next key's value in its binade
 // of 1024 keys.
+__device__ __forceinline__ int binade_of(unsigned int key) {
+  return static_cast<int>((key >= 0x8000u ? key : 0x7fffu - key) >> 10 & 31u);
+}
+__device__ __forceinline__ double step_of(int binade) { return -exp2_of(max(binade, 1) - 25); }
 __device__ __forceinline__ double value_of(unsigned int key, double& step) {
   const unsigned int bits = key >= 0x8000u ? key : 0x7fffu - key;
-  const int binade = static_cast<int>(bits >> 10 & 31u);
+  const int binade = binade_of(key);
   const unsigned int whole = (bits & 1023u) + (binade ? 1024u : 0u);
-  const double ulp = exp2_of(max(binade, 1) - 25);
-  step = -ulp;
-  return as_double(whole) * ((bits & 0x8000u) ? -ulp : ulp);
+  step = step_of(binade);
+  return as_double(whole) * ((bits & 0x8000u) ? step : -step);
 }
 
 // exp(x) for -700 <= x <= 0, without a branch, so that several run interleaved: x =
@@ -118,8 +140,8 @@ __device__ __forceinline__ double exp_above_700(double x) {
 
 // The weights of neighbouring keys of one binade: key first + e weighs
 // base * ratio^(e - shift) from e = shift on and nothing before, where shift > 0 only
-// if first lies above the row's largest logit. Two exponentials for 8 or 32 weights,
-// each within 2^-47 of exp((value - peak) / temp).
+// if first lies above the row's largest logit. One exponential and the binade's ratio for
+// 8 or 32 weights, each within 2^-47 of exp((value - peak) / temp).
 struct Weights {
   double base;
   int shift;
@@ -130,15 +152,19 @@ struct Scale {
   unsigned int top;      // the row's smallest key
   double peak, inv_temp; // its value, 1 / temperature
 
-  // the weights of two neighbouring keys of first's binade, one by the other
-  __device__ __forceinline__ double ratio(unsigned int first) const {
-    double step;
-    value_of(first, step);
-    const double x = step * inv_temp;
-    return top < kFirstFinite || first >= kMinusInf || x < -700.0 ? 0.0 : exp_above_700(fmax(x, -700.0));
+  // the weights of two neighbouring keys of a binade, one by the other, and its powers
+  __device__ __forceinline__ Ratios ratios(int binade) const {
+    const double x = step_of(binade) * inv_temp;
+    Ratios r;
+    r.r1 = x < -700.0 ? 0.0 : exp_above_700(fmin(fmax(x, -700.0), 0.0));
+    r.r2 = r.r1 * r.r1;
+    r.r4 = r.r2 * r.r2;
+    r.r8 = r.r4 * r.r4;
+    r.r16 = r.r8 * r.r8;
+    return r;
   }
 
-  __device__ __forceinline__ Weights from(unsigned int first, double keys = 8.0) const {
+  __device__ __forceinline__ Weights from(unsigned int first, double keys) const {
     const unsigned int at = max(first, top);
     double step;
     const double x = (value_of(at, step) - peak) * inv_temp;
@@ -157,16 +183,19 @@ struct Scale {
   }
 };
 
-// Counters of keys [8 j, 8 j + 8) summed over the cluster, from part `first` on (each
-// part begins with its own, so that no part is read by all at once).
+// Counters of keys [8 j, 8 j + 8), of every part from part `first` on (each part begins with
+// its own, so that no part is read by all at once) ...
 template <int kParts>
-__device__ __forceinline__ void counts8(cg::cluster_group& cluster, Shared* sh, int first, int j,
-                                        unsigned int (&c)[8]) {
-  uint4 u[kParts];
+__device__ __forceinline__ void load8(cg::cluster_group& cluster, Shared* sh, int first, int j,
+                                      uint4 (&u)[kParts]) {
 #pragma unroll
   for (int r = 0; r < kParts; ++r)
     u[r] = reinterpret_cast<const uint4*>(
         cluster.map_shared_rank(sh->hist, (first + r) % kParts))[j];
+}
+// ... and summed.
+template <int kParts>
+__device__ __forceinline__ void sum8(const uint4 (&u)[kParts], unsigned int (&c)[8]) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) c[e] = 0;
 #pragma unroll
@@ -180,20 +209,32 @@ __device__ __forceinline__ void counts8(cg::cluster_group& cluster, Shared* sh, 
   }
 }
 
-__device__ __forceinline__ double warp_scan(double v, int lane) {  // inclusive
+// c moved down by n places (0 <= n < 8), with zeros behind.
+__device__ __forceinline__ void drop(unsigned int (&c)[8], int n) {
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const double x = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += x;
+  for (int b = 1; b < 8; b <<= 1) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (n & b) c[e] = e + b < 8 ? c[e + b] : 0u;
   }
-  return v;
 }
 
-__device__ __forceinline__ int warp_scan(int v, int lane) {
+// sum over e of c[e] * r^e, in a tree (a step of fp64 takes longer than the whole tree's issue)
+__device__ __forceinline__ double weighted(const unsigned int (&c)[8], const Ratios& r) {
+  const double a = fma(r.r1, as_double(c[1]), as_double(c[0]));
+  const double b = fma(r.r1, as_double(c[3]), as_double(c[2]));
+  const double d = fma(r.r1, as_double(c[5]), as_double(c[4]));
+  const double e = fma(r.r1, as_double(c[7]), as_double(c[6]));
+  return fma(r.r4, fma(r.r2, e, d), fma(r.r2, b, a));
+}
+
+// Inclusive sums over the lanes of each group of kLanes.
+template <int kLanes = 32, typename T>
+__device__ __forceinline__ T warp_scan(T v, int lane) {
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int x = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += x;
+  for (int o = 1; o < kLanes; o <<= 1) {
+    const T x = __shfl_up_sync(0xffffffffu, v, o, kLanes);
+    if (lane % kLanes >= o) v += x;
   }
   return v;
 }
@@ -217,8 +258,10 @@ struct Query {
   }
   // how many of a key's c tokens, w each, behind t tokens of mass m (1 .. c; 1 for a NaN)
   __device__ __forceinline__ int within(int t, double m, double w, int c) const {
+    if (c == 1) return 1;
+    if (by_count) return max(1, min(count - t, c));
     const double q = (mass - m) / w;
-    const double n = by_count ? static_cast<double>(count - t) : or_equal ? floor(q) + 1.0 : ceil(q);
+    const double n = or_equal ? floor(q) + 1.0 : ceil(q);
     return n >= c ? c : n > 1.0 ? static_cast<int>(n) : 1;
   }
 };
@@ -233,43 +276,44 @@ struct Place {
   double weight;
 };
 
-// Where several parts add up a chunk's counters, the sums stay with the part that did
-// (chunk top / 256 + i with part i mod kParts, 1 KiB each behind its Shared).
-template <int kParts>
-constexpr int kSumBytes = kParts >= 4 ? kChunks / kParts * 256 * 4 : 0;
-
 // The search of one row, by one warp of CTA 0, descending from groups of 8 chunks to
-// chunks, to 8 neighbouring keys and to a key, a lane for each. A warp alone runs at the
-// pace at which its instructions are fetched, so all queries share this code.
+// chunks, entries and keys, a lane for each. A warp alone runs at the pace at which its
+// instructions are fetched, so all queries share this code.
 template <int kParts>
 struct Search {
   cg::cluster_group& cluster;
   Shared* sh;
   int lane;
-  Scale scale;
+  unsigned int top;
   int group_n, group_t;   // tokens of chunks 8 lane .. 8 lane + 7, and of all before
   double group_m;         // their mass before
 
   // Tokens and mass before every chunk; returns the row's mass.
   __device__ __forceinline__ double prefixes() {
-    group_n = 0;
-    double m = 0.0;
+    int n[8];
+    double x[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      group_n += sh->count[8 * lane + e];
-      m += sh->mass[8 * lane + e];
+      n[e] = sh->count[8 * lane + e];
+      x[e] = sh->mass[8 * lane + e];
     }
+    const double s01 = x[0] + x[1], s23 = x[2] + x[3], s45 = x[4] + x[5], s67 = x[6] + x[7];
+    const double s03 = s01 + s23, s05 = s03 + s45;
+    const double in[8] = {0.0, x[0], s01, s01 + x[2], s03, s03 + x[4], s05, s05 + x[6]};
+    const double through = warp_scan(s03 + (s45 + s67), lane);
+    const double all = __shfl_sync(0xffffffffu, through, 31);
+    const double m = __shfl_up_sync(0xffffffffu, through, 1);
+    group_m = lane == 0 ? 0.0 : m;
+    group_n = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) group_n += n[e];
     group_t = warp_scan(group_n, lane) - group_n;
-    const double through = warp_scan(m, lane), all = __shfl_sync(0xffffffffu, through, 31);
-    group_m = lane == 0 ? 0.0 : through - m;
     int t = group_t;
-    m = group_m;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       sh->before[8 * lane + e] = t;
-      sh->mass_before[8 * lane + e] = m;
-      t += sh->count[8 * lane + e];
-      m += sh->mass[8 * lane + e];
+      sh->mass_before[8 * lane + e] = group_m + in[e];
+      t += n[e];
     }
     __syncwarp();
     return all;
@@ -285,78 +329,43 @@ struct Search {
   // The last token of which the query holds.
   __device__ __forceinline__ Place last(const Query& query) const {
     const int group = pick(query, group_n > 0, group_t, group_m, 0);
-    // 8 chunks
+    // its 8 chunks
     const int at = 8 * group + (lane & 7);
-    int t = sh->before[at];
+    int n = sh->count[at], t = sh->before[at];
     double m = sh->mass_before[at];
     const int t0 = __shfl_sync(0xffffffffu, group_t, group);
-    int from = pick(query, lane < 8 && sh->count[at] > 0, t, m, t0);
+    int from = pick(query, lane < 8 && n > 0, t, m, t0);
     const int chunk = 8 * group + from;
-    const int t1 = __shfl_sync(0xffffffffu, t, from);
+    const int t1 = __shfl_sync(0xffffffffu, t, from), through1 = t1 + __shfl_sync(0xffffffffu, n, from);
     const double m1 = __shfl_sync(0xffffffffu, m, from);
-    // 32 times 8 keys
-    unsigned int c[8];
-    if (kParts >= 4) {
-      const int i = chunk - static_cast<int>(scale.top >> 8);
-      const uint4* sums = reinterpret_cast<const uint4*>(
-          cluster.map_shared_rank(reinterpret_cast<uint32_t*>(sh + 1), i % kParts) +
-          i / kParts * 256 + 8 * lane);
-      const uint4 a = sums[0], b = sums[1];
-      c[0] = a.x, c[1] = a.y, c[2] = a.z, c[3] = a.w;
-      c[4] = b.x, c[5] = b.y, c[6] = b.z, c[7] = b.w;
-    } else {
-      counts8<kParts>(cluster, sh, 0, chunk * 32 + lane, c);
-    }
-    const unsigned int first = chunk * 256 + 8 * lane;
-    const double ratio = scale.ratio(first);
-    const Weights g = scale.from(first);
-    double base = g.base;
-    if (g.tiny) base = scale.exact(first);
-    int n = 0;
-    double x = 0.0;
-#pragma unroll
-    for (int e = 7; e >= 0; --e) {
-      n += c[e];
-      if (e >= g.shift) x = fma(x, ratio, as_double(c[e]));
-    }
-    x *= base;
-    t = t1 + warp_scan(n, lane) - n;
-    m = m1;
-    {
-      const double through = warp_scan(x, lane);
-      if (lane > 0) m += through - x;
-    }
-    from = pick(query, n > 0, t, m, t1);
-    // the 8 keys of that lane
+    // the chunk's 8 entries
+    t = t1 + sh->entry_count[8 * chunk + (lane & 7)];
+    m = m1 + sh->entry_mass[8 * chunk + (lane & 7)];
+    const int behind = __shfl_down_sync(0xffffffffu, t, 1);
+    from = pick(query, lane < 8 && (lane == 7 ? through1 : behind) > t, t, m, t1);
+    const unsigned int entry = 8 * chunk + from;
     const int t2 = __shfl_sync(0xffffffffu, t, from);
     const double m2 = __shfl_sync(0xffffffffu, m, from);
-    base = __shfl_sync(0xffffffffu, base, from);
-    const int up = (lane & 7) - __shfl_sync(0xffffffffu, g.shift, from);
+    // the entry's 32 keys
+    const unsigned int key = 32 * entry + lane;
     n = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int v = __shfl_sync(0xffffffffu, static_cast<int>(c[e]), from);
-      if (lane == e) n = v;
-    }
-    const double r2 = ratio * ratio;
-    double w = up & 1 ? base * ratio : base;
-    if (up & 2) w *= r2;
-    if (up & 4) w *= r2 * r2;
-    if (up < 0) w = 0.0;
-    x = n * w;
+    for (int r = 0; r < kParts; ++r)
+      n += reinterpret_cast<const unsigned short*>(cluster.map_shared_rank(sh->hist, r))[key];
+    const int up = static_cast<int>(key - max(32 * entry, top));
+    double w = 0.0;
+    if (up >= 0) w = sh->entry_base[entry] * sh->ratios[binade_of(key)].power(up);
+    const double through = warp_scan(as_double(n) * w, lane);
+    m = __shfl_up_sync(0xffffffffu, through, 1);
+    m = lane == 0 ? m2 : m2 + m;
     t = t2 + warp_scan(n, lane) - n;
-    m = m2;
-    {
-      const double through = warp_scan(x, lane);
-      if (lane > 0) m += through - x;
-    }
-    const int k = pick(query, n > 0, t, m, t2);
-    n = __shfl_sync(0xffffffffu, n, k);
-    t = __shfl_sync(0xffffffffu, t, k);
-    m = __shfl_sync(0xffffffffu, m, k);
-    w = __shfl_sync(0xffffffffu, w, k);
+    from = pick(query, n > 0, t, m, t2);
+    n = __shfl_sync(0xffffffffu, n, from);
+    t = __shfl_sync(0xffffffffu, t, from);
+    m = __shfl_sync(0xffffffffu, m, from);
+    w = __shfl_sync(0xffffffffu, w, from);
     const int r = query.within(t, m, w, n) - 1;
-    return Place{t + r, m + r * w, static_cast<unsigned int>(chunk * 256 + 8 * from + k), r, w};
+    return Place{t + r, m + r * w, 32 * entry + from, r, w};
   }
 };
 
@@ -384,7 +393,6 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
   const float p32 = p.top_p ? p.top_p[r] : 1.f, m32 = p.min_p ? p.min_p[r] : 0.f;
   const int64_t k64 = p.top_k ? p.top_k[r] : 0;
   cluster.barrier_arrive();  // (this CTA runs: the others may write its shared memory)
-  constexpr int kUnroll = 4;
   uint4 u[kUnroll];  // the first tokens are on their way while the counters are cleared
   auto fetch = [&](int i) {
 #pragma unroll
@@ -451,6 +459,8 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
       to->bottoms[part] = sh->bottom;
     }
   }
+  const double inv_temp = 1.0 / static_cast<double>(t32);
+  if (warp == 1) sh->ratios[lane] = Scale{0u, 0.0, inv_temp}.ratios(lane);
   cluster.sync();
   top = kKeys;
 #pragma unroll
@@ -461,24 +471,43 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
 
   const bool greedy = !(t32 > 0.f) || top == 0u || top >= kMinusInf;  // uniform over the cluster
   double step;
-  const Scale scale{top, value_of(top, step), 1.0 / static_cast<double>(t32)};
+  const Scale scale{top, value_of(top, step), inv_temp};
   if (!greedy) {
     // ---- 2. tokens and mass of every chunk of keys that occur ---------------------
     const double min_p = static_cast<double>(m32);
+    const bool filter = !(m32 <= 0.f);  // (a NaN keeps nothing but the first token)
     Shared* sh0 = cluster.map_shared_rank(sh, 0);
     // A lane sums up kGroup neighbouring keys, the lanes of a chunk together. Parts of a
     // row on SMs of their own have warps to spare and wait for each other's counters: 8
-    // keys a lane there, a chunk a warp; 32 keys a lane, a binade a warp, else.
-    constexpr int kGroup = kParts >= 4 ? 8 : 32, kLanes = 256 / kGroup;
+    // keys a lane there, a chunk a warp, the next chunk's counters on their way; 32 keys a
+    // lane, a binade a warp, else.
+    constexpr bool kAhead = kParts >= 4;
+    constexpr int kGroup = kAhead ? 8 : 32, kLanes = 256 / kGroup;
+    constexpr unsigned int kStep = kParts * (kThreads / 32);
+    unsigned int unit = (top >> 8) / (kGroup / 8) + part + kParts * warp;
+    const unsigned int units = (bottom >> 8) / (kGroup / 8) + 1;
+    uint4 next[kParts];
+    if (kAhead && unit < units) load8<kParts>(cluster, sh, part, unit * 32 + lane, next);
 #pragma unroll 1
-    for (unsigned int unit = (top >> 8) / (kGroup / 8) + part + kParts * warp;
-         unit <= (bottom >> 8) / (kGroup / 8); unit += kParts * (kThreads / 32)) {
+    for (; unit < units; unit += kStep) {
       const unsigned int first = (unit * 32 + lane) * kGroup;
-      const double ratio = scale.ratio(first), r2 = ratio * ratio, r4 = r2 * r2, r8 = r4 * r4;
+      uint4 now[kParts];
+      if (kAhead) {
+#pragma unroll
+        for (int r = 0; r < kParts; ++r) now[r] = next[r];
+        if (unit + kStep < units)
+          load8<kParts>(cluster, sh, part, (unit + kStep) * 32 + lane, next);
+      }
+      const Ratios ratios = sh->ratios[binade_of(first)];
       const Weights g = scale.from(first, kGroup);
       double base = g.base;
       if (g.tiny) base = scale.exact(first);
-      const bool careful = m32 > 0.f || m32 != m32 || __any_sync(0xffffffffu, g.tiny);
+      // weights fall along a lane's keys: min-p keeps all of them, none, or (rarely) some
+      const double least = base * (kGroup == 8 ? ratios.r8 : ratios.r16 * ratios.r16);
+      const bool above_all = !filter || base >= min_p;
+      const bool careful = __any_sync(
+          0xffffffffu, g.tiny || (filter && base >= min_p && !(least > min_p * (1.0 + 1e-9))));
+      const bool at_top = __any_sync(0xffffffffu, g.shift > 0);
       int n = 0, above = 0;
       double m = 0.0, ma = 0.0;
 #pragma unroll
@@ -486,62 +515,60 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
         // lanes start at different eights: rows of 64 bytes otherwise share banks
         const int i = (j + (lane >> 1)) & (kGroup / 8 - 1);
         unsigned int c[8];
-        counts8<kParts>(cluster, sh, part, static_cast<int>(first >> 3) + i, c);
-        if (kParts >= 4) {
-          uint4* sums = reinterpret_cast<uint4*>(reinterpret_cast<uint32_t*>(sh + 1) +
-                                                 (unit - (top >> 8)) / kParts * 256 + 8 * lane);
-          sums[0] = make_uint4(c[0], c[1], c[2], c[3]);
-          sums[1] = make_uint4(c[4], c[5], c[6], c[7]);
+        if (!kAhead) load8<kParts>(cluster, sh, part, static_cast<int>(first >> 3) + i, now);
+        sum8<kParts>(now, c);
+        double x = base;  // weight of key 8 i of the group, or of the largest logit behind it
+        if (kGroup > 8 && !at_top) x *= (i & 1 ? ratios.r8 : 1.0) * (i & 2 ? ratios.r16 : 1.0);
+        if (at_top) {
+          x *= ratios.power(max(8 * i - g.shift, 0));
+          drop(c, min(max(g.shift - 8 * i, 0), 7));  // (no tokens above the largest logit)
         }
-        // x: weight of key 8 i of the group, then of the next keys
-        double x = base;
-        if (kGroup > 8) {
-          const int up = max(8 * i - g.shift, 0);
-          if (up & 1) x *= ratio;
-          if (up & 2) x *= r2;
-          if (up & 4) x *= r4;
-          if (up & 8) x *= r8;
-          if (up & 16) x *= r8 * r8;
-        }
-        if (!careful) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            n += c[e];
-            m = fma(as_double(c[e]), x, m);
-            if (8 * i + e >= g.shift) x *= ratio;
-          }
+        for (int e = 0; e < 8; ++e) n += c[e];
+        if (!careful) {
+          m = fma(weighted(c, ratios), x, m);
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            n += c[e];
             const double y = as_double(c[e]) * x;
             m += y;
-            if (x > 0.0 && x >= min_p) {
+            if (x > 0.0 && (!filter || x >= min_p)) {
               above += c[e];
               ma += y;
             }
-            if (8 * i + e >= g.shift) x *= ratio;
+            x *= ratios.r1;
           }
         }
       }
-      if (!careful) {
+      if (!careful && above_all) {
         above = n;
         ma = m;
       }
-#pragma unroll
-      for (int o = kLanes / 2; o > 0; o >>= 1) {
-        m += __shfl_xor_sync(0xffffffffu, m, o);
-        ma += __shfl_xor_sync(0xffffffffu, ma, o);
-        n += __shfl_xor_sync(0xffffffffu, n, o);
-        above += __shfl_xor_sync(0xffffffffu, above, o);
+      // what comes before each entry, and the chunk's sums
+      const int through = warp_scan<kLanes>(n, lane);
+      const double mass = warp_scan<kLanes>(m, lane);
+      double before = __shfl_up_sync(0xffffffffu, mass, 1);
+      if (lane % kLanes == 0) before = 0.0;
+      if (kGroup == 32 || lane % 4 == 0) {
+        sh0->entry_base[first >> 5] = base;
+        sh0->entry_mass[first >> 5] = before;
+        sh0->entry_count[first >> 5] = through - n;
       }
-      if (lane % kLanes == 0) {
+      if (filter || careful) {
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o >>= 1) {
+          ma += __shfl_xor_sync(0xffffffffu, ma, o);
+          above += __shfl_xor_sync(0xffffffffu, above, o);
+        }
+      }
+      if (lane % kLanes == kLanes - 1) {
         const int chunk = static_cast<int>(first >> 8);
-        sh0->mass[chunk] = m;
-        sh0->count[chunk] = n;
-        sh0->mass_above[chunk] = ma;
-        sh0->above[chunk] = above;
-        if (above < n) sh0->some = 1;
+        const bool all = !(filter || careful);
+        sh0->mass[chunk] = mass;
+        sh0->count[chunk] = through;
+        sh0->mass_above[chunk] = all ? mass : ma;
+        sh0->above[chunk] = all ? through : above;
+        if (!all && above < through) sh0->some = 1;
       }
     }
     cluster.sync();
@@ -552,7 +579,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
     unsigned int key = top;
     int rank = 0;
     if (!greedy) {
-      Search<kParts> s{cluster, sh, lane, scale};
+      Search<kParts> s{cluster, sh, lane, top};
       // kept: tokens of the shortest prefix so far, and its mass
       double all = s.prefixes(), mass = all;
       int kept = p.vocab;
@@ -613,26 +640,52 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
   const unsigned int key = sh->key;
   int rank = sh->rank;
   if (rank < 0) return;
-  // a tile of tokens in order, one group per thread: bit e of `hit` says that token
-  // first + e of the row has the key. Counts the rank down; done below zero.
-  auto tile = [&](unsigned int hit, int first) {
-    const int n = __popc(hit), through = warp_scan(n, lane);
-    __syncthreads();  // (the last tile's sums have been read)
-    if (lane == 31) sh->warp_sum[warp] = through;
-    __syncthreads();
-    const int sum = lane < kThreads / 32 ? sh->warp_sum[lane] : 0;
-    const int before = __reduce_add_sync(0xffffffffu, lane < warp ? sum : 0);
-    const int here = rank - before - (through - n);
-    if (here >= 0 && here < n) {
-      for (int e = 0; e < here; ++e) hit &= hit - 1;
-      p.out[r] = first + __ffs(hit) - 1;
+  // kUnroll tiles of tokens in order, one group per thread and tile: bit e of hit[k] says
+  // that token first + e of the row has the key, first = at + 8 (k kThreads + thread). Counts
+  // the rank down; done below zero.
+  int turn = 0;
+  auto tiles = [&](const unsigned int (&hit)[kUnroll], int at, int width) {
+    int* hits = sh->hits[turn & 1];  // (warps are at most one turn apart)
+    ++turn;
+#pragma unroll
+    for (int k = 0; k < kUnroll; ++k) {
+      const int n = __reduce_add_sync(0xffffffffu, __popc(hit[k]));
+      if (lane == 0) hits[k * (kThreads / 32) + warp] = n;
     }
-    rank -= __reduce_add_sync(0xffffffffu, sum);
+    __syncthreads();
+    static_assert(kUnroll * kThreads / 32 == 64, "two tiles of a warp per lane");
+    const int2 two = reinterpret_cast<const int2*>(hits)[lane];
+    const int through = warp_scan(two.x + two.y, lane);
+    const int all = __shfl_sync(0xffffffffu, through, 31);
+    if (rank < all) {
+      const int l = __ffs(__ballot_sync(0xffffffffu, through > rank)) - 1;
+      const int before = __shfl_sync(0xffffffffu, through - two.x - two.y, l);
+      const int x = __shfl_sync(0xffffffffu, two.x, l);
+      const bool second = rank >= before + x;
+      const int which = 2 * l + second;
+      if (which % (kThreads / 32) == warp) {
+        const int k = which / (kThreads / 32);
+        unsigned int h = 0;
+#pragma unroll
+        for (int q = 0; q < kUnroll; ++q)
+          if (q == k) h = hit[q];
+        const int n = __popc(h);
+        const int here = rank - before - (second ? x : 0) - (warp_scan(n, lane) - n);
+        if (here >= 0 && here < n) {
+          for (int e = 0; e < here; ++e) h &= h - 1;
+          p.out[r] = at + width * (k * kThreads + static_cast<int>(threadIdx.x)) + __ffs(h) - 1;
+        }
+      }
+    }
+    rank -= all;
   };
   auto is_key = [&](unsigned int bits) -> unsigned int { return key_of(bits & 0xffffu) == key; };
   fetch(threadIdx.x);
-  if (head > 0)
-    tile(threadIdx.x < head && is_key(__half_as_ushort(row[lo + threadIdx.x])), lo + threadIdx.x);
+  if (head > 0) {
+    const unsigned int hit[kUnroll] = {
+        static_cast<int>(threadIdx.x) < head && is_key(__half_as_ushort(row[lo + threadIdx.x]))};
+    tiles(hit, lo, 1);
+  }
   for (int i0 = 0; i0 < n8 && rank >= 0; i0 += kUnroll * kThreads) {
     unsigned int hit[kUnroll];
 #pragma unroll
@@ -646,21 +699,19 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
       }
     }
     fetch(i0 + kUnroll * kThreads + threadIdx.x);
-#pragma unroll
-    for (int k = 0; k < kUnroll; ++k)
-      if (rank >= 0 && i0 + k * kThreads < n8)
-        tile(hit[k], lo + head + 8 * (i0 + k * kThreads + static_cast<int>(threadIdx.x)));
+    tiles(hit, lo + head + 8 * i0, 8);
   }
   if (rank >= 0 && tail > 0) {
-    const int i = 8 * n8 + static_cast<int>(threadIdx.x);
-    tile(threadIdx.x < tail && is_key(__half_as_ushort(body[i])), lo + head + i);
+    const unsigned int hit[kUnroll] = {static_cast<int>(threadIdx.x) < tail &&
+                                       is_key(__half_as_ushort(body[8 * n8 + threadIdx.x]))};
+    tiles(hit, lo + head + 8 * n8, 1);
   }
 }
 
 template <int kParts>
 int launch(const Params& p, int64_t rows, int slot, cudaStream_t stream) {
   const int st = ensure_smem_attribute(reinterpret_cast<const void*>(&sample_kernel<kParts>),
-                                       static_cast<int>(sizeof(Shared)) + kSumBytes<kParts>, slot);
+                                       sizeof(Shared), slot);
   if (st != CIE_OK) return st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -670,7 +721,7 @@ int launch(const Params& p, int64_t rows, int slot, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(rows * kParts));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = sizeof(Shared) + kSumBytes<kParts>;
+  cfg.dynamicSmemBytes = sizeof(Shared);
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
