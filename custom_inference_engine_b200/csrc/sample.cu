@@ -11,7 +11,12 @@
 //
 // One cluster of C CTAs per row, C parts of the row:
 //   1. every CTA counts its part into 2^16 16-bit counters in its shared memory
-//      (two to a word, 128 KiB; a part has at most 65528 tokens, so none overflows);
+//      (two to a word, 128 KiB). The most frequent of a sample of 32 tokens is counted in
+//      registers instead: in a masked row most tokens are alike, and atomics on one
+//      address take turns (99 % of a row masked: 68 us for 64 rows of 151936 without
+//      this, no more than other rows with it). Parts of up to 98296 tokens save waves of CTAs (64
+//      rows of 151936: 35 us as 4 parts a row, 22 us as 2); at most one key of such a part has
+//      65536 tokens or more, and its counter is kept less 65536 with the key noted;
 //   2. the keys form 256 chunks of 8 entries of 32 keys (an entry lies in one binade, so its
 //      weights are a geometric sequence); warps sum the counters over the cluster
 //      (distributed shared memory) and hand CTA 0 each chunk's tokens, mass and tokens
@@ -25,6 +30,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "cie_host.h"
 #include "cie_model_ops.h"
 
@@ -37,9 +44,12 @@ constexpr int kThreads = 512;
 constexpr int kKeys = 1 << 16;
 constexpr int kChunks = 256;              // of 8 entries
 constexpr int kEntries = 8 * kChunks;     // of 32 keys
-constexpr int kUnroll = 4;                // 16-byte units of the row in flight per thread
-constexpr int kMaxPart = 65528;           // tokens of a part: multiple of 8 below 2^16
+constexpr int kUnroll = 8;                // 16-byte units of the row in flight per thread
+constexpr int kMaxPart = 98296;           // tokens of a part: multiple of 8 below 1.5 * 2^16
 constexpr int kMaxCluster = 8;
+constexpr int kMaxVocab = 524224;
+constexpr unsigned int kNone = 0xffffffffu;  // no key
+constexpr int kOften = 4;  // of 32 sampled tokens: the key is counted apart
 // keys of some values
 constexpr unsigned int kPlusInf = 0x3FF, kFirstFinite = 0x400, kPlusZero = 0x7FFF;
 constexpr unsigned int kMinusZero = 0x8000, kMinusInf = 0xFC00;
@@ -80,11 +90,18 @@ struct alignas(16) Shared {
   int entry_count[kEntries];
   int count[kChunks], before[kChunks], above[kChunks];
   int some;
-  alignas(8) int hits[2][kUnroll * kThreads / 32];
+  alignas(16) int hits[2][kUnroll * kThreads / 32];
   unsigned int top, bottom;       // smallest and largest key of this CTA's part
-  unsigned int tops[kMaxCluster], bottoms[kMaxCluster];  // and of every part
+  unsigned int often;             // the key that is counted in registers
+  unsigned int extra;             // the key whose counter lacks 65536
+  int run, pairs;                 // tokens of key `often`; pairs of equal other ones
+  // of every part
+  unsigned int tops[kMaxCluster], bottoms[kMaxCluster], extras[kMaxCluster];
   unsigned int key;               // the sampled token's key and its rank among this
   int rank;                       // part's tokens of that key (negative: not here)
+  int tokens;                     // how many those are
+  int found;                      // tokens listed so far
+  int list[kThreads];
 };
 
 // Ordered keys of two fp16 values: descending values ascend, NaNs lie below +inf's key
@@ -209,6 +226,18 @@ __device__ __forceinline__ void sum8(const uint4 (&u)[kParts], unsigned int (&c)
   }
 }
 
+// Adds the 65536 that a part's counter of one of the keys [first, first + 8) may lack.
+template <int kParts>
+__device__ __forceinline__ void add_extras(const Shared* sh, unsigned int first,
+                                           unsigned int (&c)[8]) {
+#pragma unroll 1
+  for (int r = 0; r < kParts; ++r) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (sh->extras[r] == first + e) c[e] += 65536u;
+  }
+}
+
 // c moved down by n places (0 <= n < 8), with zeros behind.
 __device__ __forceinline__ void drop(unsigned int (&c)[8], int n) {
 #pragma unroll
@@ -285,6 +314,7 @@ struct Search {
   Shared* sh;
   int lane;
   unsigned int top;
+  bool extras;            // some counter lacks 65536
   int group_n, group_t;   // tokens of chunks 8 lane .. 8 lane + 7, and of all before
   double group_m;         // their mass before
 
@@ -352,6 +382,10 @@ struct Search {
 #pragma unroll
     for (int r = 0; r < kParts; ++r)
       n += reinterpret_cast<const unsigned short*>(cluster.map_shared_rank(sh->hist, r))[key];
+    if (extras) {
+#pragma unroll 1
+      for (int r = 0; r < kParts; ++r) n += sh->extras[r] == key ? 65536 : 0;
+    }
     const int up = static_cast<int>(key - max(32 * entry, top));
     double w = 0.0;
     if (up >= 0) w = sh->entry_base[entry] * sh->ratios[binade_of(key)].power(up);
@@ -400,71 +434,130 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
       if (i + k * kThreads < n8) u[k] = row8[i + k * kThreads];
   };
   fetch(threadIdx.x);
+  uint32_t sample = kNone;  // one of 32 tokens spread over the part
+  if (warp == 0 && hi > lo)
+    sample = __half_as_ushort(row[lo + static_cast<int>((hi - lo) * int64_t(lane) >> 5)]);
   for (int i = threadIdx.x; i < kKeys / 8; i += kThreads)
     reinterpret_cast<uint4*>(sh->hist)[i] = make_uint4(0, 0, 0, 0);
   if (threadIdx.x < kChunks) {
     sh->count[threadIdx.x] = sh->above[threadIdx.x] = 0;
     sh->mass[threadIdx.x] = sh->mass_above[threadIdx.x] = 0.0;
   }
-  if (threadIdx.x == 0) {
-    sh->top = kKeys;
-    sh->bottom = sh->some = 0;
+  if (warp == 0) {
+    const int times = __popc(__match_any_sync(0xffffffffu, sample));
+    const int best = __reduce_max_sync(0xffffffffu, times << 5 | lane);
+    uint32_t k = __shfl_sync(0xffffffffu, sample, best & 31);
+    k = best >> 5 < kOften || k == kNone ? kNone : keys_of2(k) & 0xffffu;
+    if (lane == 0) {
+      sh->often = k;
+      sh->extra = kNone;
+      sh->top = kKeys;
+      sh->bottom = sh->some = sh->run = sh->pairs = sh->found = 0;
+    }
   }
   __syncthreads();
+  const unsigned int often = sh->often;
+  int run = 0, pairs = 0;
   uint32_t top2 = 0xffffffffu, bottom2 = 0u;  // of even and odd tokens
-  auto count = [&](unsigned int key) { atomicAdd(&sh->hist[key >> 1], (key & 1u) * 0xffffu + 1u); };
-  auto count2 = [&](uint32_t bits) {
-    const uint32_t k = keys_of2(bits);
-    top2 = __vminu2(top2, k);
-    bottom2 = __vmaxu2(bottom2, k);
-    count(k & 0xffffu);
-    count(k >> 16);
+  auto step_at = [](unsigned int key) { return (key & 1u) * 0xffffu + 1u; };
+  // a comparison per token costs half of the loop's speed again: only where it pays
+  auto count = [&](auto apart, unsigned int key) {
+    if (decltype(apart)::value && key == often) ++run;
+    else atomicAdd(&sh->hist[key >> 1], step_at(key));
   };
-  for (int i = threadIdx.x; i < n8; i += kUnroll * kThreads) {
+  auto count_all = [&](auto apart, auto wide) {
+    auto count2 = [&](uint32_t bits) {
+      const uint32_t k = keys_of2(bits);
+      top2 = __vminu2(top2, k);
+      bottom2 = __vmaxu2(bottom2, k);
+      const unsigned int a = k & 0xffffu, b = k >> 16;
+      if (decltype(wide)::value) pairs += a == b && !(decltype(apart)::value && b == often);
+      count(apart, a);
+      count(apart, b);
+    };
+    for (int i = threadIdx.x; i < n8; i += kUnroll * kThreads) {
 #pragma unroll
-    for (int k = 0; k < kUnroll; ++k) {
-      if (i + k * kThreads >= n8) break;
-      count2(u[k].x);
-      count2(u[k].y);
-      count2(u[k].z);
-      count2(u[k].w);
+      for (int k = 0; k < kUnroll; ++k) {
+        if (i + k * kThreads >= n8) break;
+        count2(u[k].x);
+        count2(u[k].y);
+        count2(u[k].z);
+        count2(u[k].w);
+      }
+      fetch(i + kUnroll * kThreads);
     }
-    fetch(i + kUnroll * kThreads);
-  }
+  };
+  if (often != kNone) count_all(std::true_type{}, std::true_type{});
+  else if (hi - lo > 65535) count_all(std::false_type{}, std::true_type{});
+  else count_all(std::false_type{}, std::false_type{});
   if (threadIdx.x < head + tail) {
     const int i = threadIdx.x < head ? static_cast<int>(threadIdx.x) - head
                                      : 8 * n8 + static_cast<int>(threadIdx.x) - head;
     const uint32_t k = keys_of2(__half_as_ushort(body[i])) & 0xffffu;
     top2 = __vminu2(top2, 0xffff0000u | k);
     bottom2 = __vmaxu2(bottom2, k);
-    count(k);
+    count(std::true_type{}, k);
   }
   unsigned int top = __reduce_min_sync(0xffffffffu, min(top2 & 0xffffu, top2 >> 16));
   unsigned int bottom = __reduce_max_sync(0xffffffffu, max(bottom2 & 0xffffu, bottom2 >> 16));
+  run = __reduce_add_sync(0xffffffffu, run);
+  pairs = __reduce_add_sync(0xffffffffu, pairs);
   if (lane == 0) {
     atomicMin(&sh->top, top);
     atomicMax(&sh->bottom, bottom);
+    atomicAdd(&sh->run, run);
+    atomicAdd(&sh->pairs, pairs);
   }
   cluster.barrier_wait();
   __syncthreads();
+  // 65536 tokens of one key among n fill at least 65536 - n / 2 of the part's pairs (16384
+  // of the largest part's): only then can a counter have run over, and the part is counted
+  // again with atomics that show it. (Two of a word never run over together.)
+  const bool again = hi - lo > 65535 && sh->pairs >= 65536 - (hi - lo + 1) / 2 - 16;
+  if (again) {
+    for (int i = threadIdx.x; i < kKeys / 8; i += kThreads)
+      reinterpret_cast<uint4*>(sh->hist)[i] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    for (int i = lo + static_cast<int>(threadIdx.x); i < hi; i += kThreads) {
+      const unsigned int k = keys_of2(__half_as_ushort(row[i])) & 0xffffu;
+      const uint32_t old = atomicAdd(&sh->hist[k >> 1], step_at(k));
+      if ((k & 1u ? old >> 16 : old & 0xffffu) == 0xffffu) {
+        if (!(k & 1u)) atomicSub(&sh->hist[k >> 1], 0x10000u);  // the carry
+        sh->extra = k;
+      }
+    }
+    __syncthreads();
+  }
   if (threadIdx.x == 0) {
+    unsigned short* counters = reinterpret_cast<unsigned short*>(sh->hist);
+    if (!again && often != kNone) {
+      counters[often] = static_cast<unsigned short>(sh->run);
+      if (sh->run >= 65536) sh->extra = often;
+    }
     // -0 counts as +0; a part with a NaN says so with key 0 at its top
-    sh->hist[kPlusZero >> 1] += (sh->hist[kMinusZero >> 1] & 0xffffu) << 16;
-    sh->hist[kMinusZero >> 1] &= 0xffff0000u;
+    const bool extra = sh->extra == kPlusZero || sh->extra == kMinusZero;
+    const int zeros = counters[kPlusZero] + counters[kMinusZero] + (extra ? 65536 : 0);
+    counters[kPlusZero] = static_cast<unsigned short>(zeros);
+    counters[kMinusZero] = 0;
+    if (zeros >= 65536) sh->extra = kPlusZero;
+    else if (extra) sh->extra = kNone;
     if (sh->top == kMinusZero) sh->top = kPlusZero;
     if (sh->top < kPlusInf || sh->bottom > kMinusInf) sh->top = 0;
     for (int q = 0; q < kParts; ++q) {
       Shared* to = cluster.map_shared_rank(sh, q);
       to->tops[part] = sh->top;
       to->bottoms[part] = sh->bottom;
+      to->extras[part] = sh->extra;
     }
   }
   const double inv_temp = 1.0 / static_cast<double>(t32);
   if (warp == 1) sh->ratios[lane] = Scale{0u, 0.0, inv_temp}.ratios(lane);
   cluster.sync();
   top = kKeys;
+  bool extras = false;
 #pragma unroll
   for (int q = 0; q < kParts; ++q) {
+    extras |= sh->extras[q] != kNone;
     top = min(top, sh->tops[q]);
     bottom = max(bottom, sh->bottoms[q]);
   }
@@ -477,33 +570,46 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
     const double min_p = static_cast<double>(m32);
     const bool filter = !(m32 <= 0.f);  // (a NaN keeps nothing but the first token)
     Shared* sh0 = cluster.map_shared_rank(sh, 0);
-    // A lane sums up kGroup neighbouring keys, the lanes of a chunk together. Parts of a
-    // row on SMs of their own have warps to spare and wait for each other's counters: 8
-    // keys a lane there, a chunk a warp, the next chunk's counters on their way; 32 keys a
-    // lane, a binade a warp, else.
+    // A lane sums up kGroup neighbouring keys, the lanes of a chunk together. Many parts
+    // have warps to spare and wait for each other's counters: 8 keys a lane there, a chunk a
+    // warp, the next chunk's counters on their way; 16 keys a lane in two parts, 32 (a binade
+    // a warp) in one.
     constexpr bool kAhead = kParts >= 4;
-    constexpr int kGroup = kAhead ? 8 : 32, kLanes = 256 / kGroup;
+    constexpr int kGroup = kParts == 1 ? 32 : kParts == 2 ? 16 : 8, kLanes = 256 / kGroup;
+    constexpr int kWords = kGroup / 8;
     constexpr unsigned int kStep = kParts * (kThreads / 32);
     unsigned int unit = (top >> 8) / (kGroup / 8) + part + kParts * warp;
     const unsigned int units = (bottom >> 8) / (kGroup / 8) + 1;
-    uint4 next[kParts];
-    if (kAhead && unit < units) load8<kParts>(cluster, sh, part, unit * 32 + lane, next);
+    uint4 next[kWords][kParts];
+    // lanes start at different eights: rows of 32 or 64 bytes otherwise share banks
+    auto eight = [&](int j) { return (j + lane * kGroup / 64) & (kWords - 1); };
+    auto load = [&](unsigned int unit) {
+#pragma unroll
+      for (int j = 0; j < kWords; ++j)
+        load8<kParts>(cluster, sh, part, (unit * 32 + lane) * kWords + eight(j), next[j]);
+    };
+    if (kAhead && unit < units) load(unit);
 #pragma unroll 1
     for (; unit < units; unit += kStep) {
       const unsigned int first = (unit * 32 + lane) * kGroup;
-      uint4 now[kParts];
-      if (kAhead) {
+      uint4 now[kWords][kParts];
+      if (!kAhead) load(unit);
+      uint32_t any = extras;
 #pragma unroll
-        for (int r = 0; r < kParts; ++r) now[r] = next[r];
-        if (unit + kStep < units)
-          load8<kParts>(cluster, sh, part, (unit + kStep) * 32 + lane, next);
-      }
+      for (int j = 0; j < kWords; ++j)
+#pragma unroll
+        for (int r = 0; r < kParts; ++r) {
+          now[j][r] = next[j][r];
+          any |= now[j][r].x | now[j][r].y | now[j][r].z | now[j][r].w;
+        }
+      if (kAhead && unit + kStep < units) load(unit + kStep);
+      if (!__any_sync(0xffffffffu, any)) continue;  // (the binades next to zero)
       const Ratios ratios = sh->ratios[binade_of(first)];
       const Weights g = scale.from(first, kGroup);
       double base = g.base;
       if (g.tiny) base = scale.exact(first);
       // weights fall along a lane's keys: min-p keeps all of them, none, or (rarely) some
-      const double least = base * (kGroup == 8 ? ratios.r8 : ratios.r16 * ratios.r16);
+      const double least = base * (kGroup == 8 ? ratios.r8 : kGroup == 16 ? ratios.r16 : ratios.r16 * ratios.r16);
       const bool above_all = !filter || base >= min_p;
       const bool careful = __any_sync(
           0xffffffffu, g.tiny || (filter && base >= min_p && !(least > min_p * (1.0 + 1e-9))));
@@ -511,12 +617,11 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
       int n = 0, above = 0;
       double m = 0.0, ma = 0.0;
 #pragma unroll
-      for (int j = 0; j < kGroup / 8; ++j) {
-        // lanes start at different eights: rows of 64 bytes otherwise share banks
-        const int i = (j + (lane >> 1)) & (kGroup / 8 - 1);
+      for (int j = 0; j < kWords; ++j) {
+        const int i = eight(j);
         unsigned int c[8];
-        if (!kAhead) load8<kParts>(cluster, sh, part, static_cast<int>(first >> 3) + i, now);
-        sum8<kParts>(now, c);
+        sum8<kParts>(now[j], c);
+        if (extras) add_extras<kParts>(sh, first + 8 * i, c);
         double x = base;  // weight of key 8 i of the group, or of the largest logit behind it
         if (kGroup > 8 && !at_top) x *= (i & 1 ? ratios.r8 : 1.0) * (i & 2 ? ratios.r16 : 1.0);
         if (at_top) {
@@ -549,7 +654,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
       const double mass = warp_scan<kLanes>(m, lane);
       double before = __shfl_up_sync(0xffffffffu, mass, 1);
       if (lane % kLanes == 0) before = 0.0;
-      if (kGroup == 32 || lane % 4 == 0) {
+      if (lane % (32 / kGroup) == 0) {
         sh0->entry_base[first >> 5] = base;
         sh0->entry_mass[first >> 5] = before;
         sh0->entry_count[first >> 5] = through - n;
@@ -574,12 +679,13 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
     cluster.sync();
   }
 
+  fetch(threadIdx.x);  // (for the look-up)
   // ---- 3. the sampled token's key and rank ---------------------------------------
   if (part == 0 && warp == 0) {
     unsigned int key = top;
     int rank = 0;
     if (!greedy) {
-      Search<kParts> s{cluster, sh, lane, top};
+      Search<kParts> s{cluster, sh, lane, top, extras};
       // kept: tokens of the shortest prefix so far, and its mass
       double all = s.prefixes(), mass = all;
       int kept = p.vocab;
@@ -624,7 +730,8 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
         c = sh->tops[lane] == 0;
       } else {
         const uint32_t w = *cluster.map_shared_rank(&sh->hist[key >> 1], lane);
-        c = static_cast<int>((key & 1u) ? w >> 16 : w & 0xffffu);
+        c = static_cast<int>((key & 1u) ? w >> 16 : w & 0xffffu) +
+            (sh->extras[lane] == key ? 65536 : 0);
       }
     }
     rank -= warp_scan(c, lane) - c;
@@ -632,6 +739,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
       Shared* to = cluster.map_shared_rank(sh, lane);
       to->key = key;
       to->rank = rank < c ? rank : -1;
+      to->tokens = c;
     }
   }
   cluster.sync();
@@ -640,6 +748,45 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
   const unsigned int key = sh->key;
   int rank = sh->rank;
   if (rank < 0) return;
+  if (key != 0 && sh->tokens <= kThreads) {
+    // Few such tokens: listed in any order, then the one that has `rank` others before it.
+    // Halves that differ from the key's bits in nothing (of a zero: nothing but the sign)
+    // show up as the sign bit that x - 1 sets in a half x without one.
+    const uint32_t mask = key == kPlusZero ? 0x7fff7fffu : 0xffffffffu;
+    const uint32_t want = (key >= 0x8000u ? key : 0x7fffu - key) * 0x00010001u;
+    auto miss = [&](uint32_t w) { return (w ^ want) & mask; };
+    auto add = [&](int at) { sh->list[atomicAdd(&sh->found, 1)] = at; };
+    for (int i = threadIdx.x; i < n8; i += kUnroll * kThreads) {
+#pragma unroll
+      for (int k = 0; k < kUnroll; ++k) {
+        if (i + k * kThreads >= n8) break;
+        const uint32_t x[4] = {miss(u[k].x), miss(u[k].y), miss(u[k].z), miss(u[k].w)};
+        uint32_t any = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) any |= (x[e] - 0x00010001u) & ~x[e];
+        if (any & 0x80008000u) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if ((x[e >> 1] >> (e & 1) * 16 & 0xffffu) == 0) add(lo + head + 8 * (i + k * kThreads) + e);
+        }
+      }
+      fetch(i + kUnroll * kThreads);
+    }
+    if (threadIdx.x < head + tail) {
+      const int i = threadIdx.x < head ? static_cast<int>(threadIdx.x) - head
+                                       : 8 * n8 + static_cast<int>(threadIdx.x) - head;
+      if ((miss(__half_as_ushort(body[i])) & 0xffffu) == 0) add(lo + head + i);
+    }
+    __syncthreads();
+    const int n = sh->tokens;
+    if (static_cast<int>(threadIdx.x) < n) {
+      const int at = sh->list[threadIdx.x];
+      int before = 0;
+      for (int i = 0; i < n; ++i) before += sh->list[i] < at;
+      if (before == rank) p.out[r] = at;
+    }
+    return;
+  }
   // kUnroll tiles of tokens in order, one group per thread and tile: bit e of hit[k] says
   // that token first + e of the row has the key, first = at + 8 (k kThreads + thread). Counts
   // the rank down; done below zero.
@@ -653,16 +800,23 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
       if (lane == 0) hits[k * (kThreads / 32) + warp] = n;
     }
     __syncthreads();
-    static_assert(kUnroll * kThreads / 32 == 64, "two tiles of a warp per lane");
-    const int2 two = reinterpret_cast<const int2*>(hits)[lane];
-    const int through = warp_scan(two.x + two.y, lane);
+    static_assert(kUnroll * kThreads / 32 == 128, "four tiles of a warp per lane");
+    const int4 four = reinterpret_cast<const int4*>(hits)[lane];
+    const int sums[4] = {four.x, four.y, four.z, four.w};
+    const int through = warp_scan(four.x + four.y + four.z + four.w, lane);
     const int all = __shfl_sync(0xffffffffu, through, 31);
     if (rank < all) {
       const int l = __ffs(__ballot_sync(0xffffffffu, through > rank)) - 1;
-      const int before = __shfl_sync(0xffffffffu, through - two.x - two.y, l);
-      const int x = __shfl_sync(0xffffffffu, two.x, l);
-      const bool second = rank >= before + x;
-      const int which = 2 * l + second;
+      int before = through - (four.x + four.y + four.z + four.w), which = 4 * lane;
+#pragma unroll
+      for (int e = 0; e < 3; ++e) {
+        if (which == 4 * lane + e && rank >= before + sums[e]) {
+          before += sums[e];
+          ++which;
+        }
+      }
+      before = __shfl_sync(0xffffffffu, before, l);
+      which = __shfl_sync(0xffffffffu, which, l);
       if (which % (kThreads / 32) == warp) {
         const int k = which / (kThreads / 32);
         unsigned int h = 0;
@@ -670,7 +824,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
         for (int q = 0; q < kUnroll; ++q)
           if (q == k) h = hit[q];
         const int n = __popc(h);
-        const int here = rank - before - (second ? x : 0) - (warp_scan(n, lane) - n);
+        const int here = rank - before - (warp_scan(n, lane) - n);
         if (here >= 0 && here < n) {
           for (int e = 0; e < here; ++e) h &= h - 1;
           p.out[r] = at + width * (k * kThreads + static_cast<int>(threadIdx.x)) + __ffs(h) - 1;
@@ -680,7 +834,6 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
     rank -= all;
   };
   auto is_key = [&](unsigned int bits) -> unsigned int { return key_of(bits & 0xffffu) == key; };
-  fetch(threadIdx.x);
   if (head > 0) {
     const unsigned int hit[kUnroll] = {
         static_cast<int>(threadIdx.x) < head && is_key(__half_as_ushort(row[lo + threadIdx.x]))};
@@ -744,8 +897,8 @@ int cie_sample_rows(const void* logits, int64_t rows, int64_t vocab, int64_t str
   if (rows == 0) return CIE_OK;
   if (!logits || !uniform || !temperature || !out || vocab == 0)
     return fail(CIE_ERR_INVALID_ARGUMENT, "null pointer or empty row");
-  if (vocab > static_cast<int64_t>(kMaxPart) * kMaxCluster)
-    return fail(CIE_ERR_UNSUPPORTED, "vocab %lld > %d", (long long)vocab, kMaxPart * kMaxCluster);
+  if (vocab > kMaxVocab)
+    return fail(CIE_ERR_UNSUPPORTED, "vocab %lld > %d", (long long)vocab, kMaxVocab);
   if (stride < vocab) return fail(CIE_ERR_INVALID_ARGUMENT, "row stride < vocab");
   if ((reinterpret_cast<uintptr_t>(logits) & 1) != 0)
     return fail(CIE_ERR_ALIGNMENT, "logits must be 2-byte aligned");

@@ -179,6 +179,45 @@ def test_constant_rows(ops, cuda_device):
         assert got.tolist() == [min(int(a * n), n - 1) for a in u.tolist()], vocab
 
 
+@pytest.mark.parametrize("rows,vocab", [(76, 98296), (76, 98289), (40, 151936), (40, 196592),
+                                        (20, 390001)])
+def test_parts_of_more_than_two_to_the_16_tokens(ops, cuda_device, rows, vocab):
+    """One token value fills most of a part: counted apart when it is found early, and found
+    by a second count when 32 evenly spread tokens of the part are others."""
+    dev, g = cuda_device, torch.Generator().manual_seed(vocab)
+    rand = lambda *n: torch.rand(*n, generator=g)
+    parts = next(c for c in (1, 2, 4, 8) if -(-vocab // (8 * c)) * 8 <= 98296)
+    part = -(-vocab // (8 * parts)) * 8
+    fill = [0.25, 0.25024414, -0.0, 0.0, -65504.0, -math.inf]  # (keys of either parity)
+    x = torch.empty(rows, vocab).half()
+    for i, value in enumerate(fill):
+        x[i] = torch.randn(vocab, generator=g) * 2.5
+        where = rand(vocab) < 0.9
+        if i % 2:  # the sampled tokens stay as they are, each twice
+            for lo in range(0, vocab, part):
+                n = min(part, vocab - lo)
+                at = torch.tensor([lo + (n * l >> 5) for l in range(32)])
+                where[at] = False
+                x[i, at] = x[i, at[:16]].repeat(2)
+        x[i, where] = value
+        if value == 0:  # zeros of both signs, fewer than 2^16 of each
+            x[i, where.nonzero()[::2, 0]] = -value
+    # exactly 65535, 65536 and 65537 tokens of one value in the first part
+    for i, n in enumerate((65535, 65536, 65537)):
+        x[6 + i] = (torch.randn(vocab, generator=g) * 2.5).half()
+        x[6 + i, torch.randperm(min(part, vocab), generator=g)[:n]] = 1.5 + i / 1024
+    x[9:] = x[8]
+    u, t = rand(rows), torch.ones(rows)
+    t[4] = 1e5  # (the lowest value keeps half of its weight)
+    k = torch.full((rows,), vocab // 2)
+    p, m = rand(rows), torch.full((rows,), 0.01)
+    for args in ((u, t), (u, t, k), (u, t, k, p, m)):
+        got = ops.sample_rows(x.to(dev), *(a.to(dev) for a in args))
+        assert got[:9].tolist() == _want(x[:9], *(a[:9] for a in args))
+        again = ops.sample_rows(x.to(dev), *(a.to(dev) for a in args))
+        assert torch.equal(got, again)
+
+
 def test_follows_the_distribution(ops, cuda_device):
     """Evenly spaced numbers over one row: the tokens' counts are their probabilities
     to within one."""
