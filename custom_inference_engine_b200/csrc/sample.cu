@@ -10,13 +10,13 @@
 // token depends on nothing but the inputs. The row is read twice and never sorted.
 //
 // One cluster of C CTAs per row, C parts of the row:
-//   1. every CTA counts its part into 2^16 16-bit counters in its shared memory
-//      (two to a word, 128 KiB). The most frequent of a sample of 32 tokens is counted in
-//      registers instead: in a masked row most tokens are alike, and atomics on one
-//      address take turns (99 % of a row masked: 68 us for 64 rows of 151936 without
-//      this, no more than other rows with it). Parts of up to 98296 tokens save waves of CTAs (64
-//      rows of 151936: 35 us as 4 parts a row, 22 us as 2); at most one key of such a part has
-//      65536 tokens or more, and its counter is kept less 65536 with the key noted;
+//   1. every CTA counts its part into 2^16 16-bit counters in its shared memory (two to a
+//      word, 128 KiB). A key that 4 of 32 sampled tokens have is counted in registers
+//      instead: in a masked row most tokens are alike, and atomics on one address take
+//      turns (64 rows of 151936, 99 % masked: 68 us without this, 25 us with it). Parts
+//      of up to 98296 tokens save waves of CTAs (64 rows of 151936: 31 us as 4 parts a row,
+//      23 us as 2); one key at most of such a part has 65536 tokens or more, and its
+//      counter is kept less 65536 with the key noted;
 //   2. the keys form 256 chunks of 8 entries of 32 keys (an entry lies in one binade, so its
 //      weights are a geometric sequence); warps sum the counters over the cluster
 //      (distributed shared memory) and hand CTA 0 each chunk's tokens, mass and tokens
@@ -24,7 +24,15 @@
 //   3. CTA 0's first warp finds the kept prefix and the key of the sampled token
 //      with its rank among the tokens of that key, descending to one entry's keys for
 //      each prefix;
-//   4. the CTA whose part holds that token looks it up in the row.
+//   4. the CTA whose part holds that token looks it up in the row, whose first tokens were
+//      loaded again during the search.
+//
+// Measured (B200, device time): one row of 151936 15 us, 64 rows 23 us, 256 rows of 32003
+// 30 us; with top-k, top-p and min-p 3 to 4 us more. What bounds it, of the 16 us of a CTA
+// that counts 75968 tokens: shared atomics on random banks 6.5 us (6 tokens a cycle), the
+// chunks' sums 4 us (fp64 latency, and distributed shared memory at about 22 bytes a cycle
+// and SM), each search 1.7 us (one warp), clearing, barriers and look-up the rest. 128 KiB of
+// counters allow one CTA per SM, so that more than 148 of them take another wave.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -101,6 +109,7 @@ struct alignas(16) Shared {
   int rank;                       // part's tokens of that key (negative: not here)
   int tokens;                     // how many those are
   int found;                      // tokens listed so far
+  unsigned int unit;              // of chunk sums, the next one to take up
   int list[kThreads];
 };
 
@@ -453,6 +462,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
       sh->extra = kNone;
       sh->top = kKeys;
       sh->bottom = sh->some = sh->run = sh->pairs = sh->found = 0;
+      sh->unit = 0;
     }
   }
   __syncthreads();
@@ -577,9 +587,8 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
     constexpr bool kAhead = kParts >= 4;
     constexpr int kGroup = kParts == 1 ? 32 : kParts == 2 ? 16 : 8, kLanes = 256 / kGroup;
     constexpr int kWords = kGroup / 8;
-    constexpr unsigned int kStep = kParts * (kThreads / 32);
-    unsigned int unit = (top >> 8) / (kGroup / 8) + part + kParts * warp;
-    const unsigned int units = (bottom >> 8) / (kGroup / 8) + 1;
+    const unsigned int unit0 = (top >> 8) / kWords + part;
+    const unsigned int units = (bottom >> 8) / kWords + 1;
     uint4 next[kWords][kParts];
     // lanes start at different eights: rows of 32 or 64 bytes otherwise share banks
     auto eight = [&](int j) { return (j + lane * kGroup / 64) & (kWords - 1); };
@@ -588,9 +597,16 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
       for (int j = 0; j < kWords; ++j)
         load8<kParts>(cluster, sh, part, (unit * 32 + lane) * kWords + eight(j), next[j]);
     };
+    // Empty units are soon done: warps take the next one when they are free.
+    constexpr unsigned int kStep = kParts * (kThreads / 32);
+    auto take = [&]() {
+      const unsigned int n = lane == 0 ? atomicAdd(&sh->unit, 1u) : 0u;
+      return unit0 + kParts * __shfl_sync(0xffffffffu, n, 0);
+    };
+    unsigned int unit = kAhead ? unit0 + kParts * warp : take();
     if (kAhead && unit < units) load(unit);
 #pragma unroll 1
-    for (; unit < units; unit += kStep) {
+    for (; unit < units; unit = kAhead ? unit + kStep : take()) {
       const unsigned int first = (unit * 32 + lane) * kGroup;
       uint4 now[kWords][kParts];
       if (!kAhead) load(unit);
