@@ -13,9 +13,9 @@
 //   1. every CTA counts its part into 2^16 16-bit counters in its shared memory (two to a
 //      word, 128 KiB). A key that 4 of 32 sampled tokens have is counted in registers
 //      instead: in a masked row most tokens are alike, and atomics on one address take
-//      turns (64 rows of 151936, 99 % masked: 68 us without this, 25 us with it). Parts
-//      of up to 98296 tokens save waves of CTAs (64 rows of 151936: 31 us as 4 parts a row,
-//      23 us as 2); one key at most of such a part has 65536 tokens or more, and its
+//      turns (64 rows of 151936, 99 % masked: 68 us without this, 23 us with it). Parts
+//      of up to 98296 tokens save waves of CTAs (64 rows of 151936: 29 us as 4 parts a row,
+//      21 us as 2); one key at most of such a part has 65536 tokens or more, and its
 //      counter is kept less 65536 with the key noted;
 //   2. the keys form 256 chunks of 8 entries of 32 keys (an entry lies in one binade, so its
 //      weights are a geometric sequence); warps sum the counters over the cluster
@@ -27,8 +27,8 @@
 //   4. the CTA whose part holds that token looks it up in the row, whose first tokens were
 //      loaded again during the search.
 //
-// Measured (B200, device time): one row of 151936 15 us, 64 rows 23 us, 256 rows of 32003
-// 30 us; with top-k, top-p and min-p 3 to 4 us more. What bounds it, of the 16 us of a CTA
+// Measured (B200, device time in a graph of calls): one row of 151936 14 us, 64 rows 21 us,
+// 256 rows of 32003 27 us; with top-k, top-p and min-p 2 to 4 us more. What bounds it, of the 16 us of a CTA
 // that counts 75968 tokens: shared atomics on random banks 6.5 us (6 tokens a cycle), the
 // chunks' sums 4 us (fp64 latency, and distributed shared memory at about 22 bytes a cycle
 // and SM), each search 1.7 us (one warp), clearing, barriers and look-up the rest. 128 KiB of
@@ -38,6 +38,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "cie_host.h"
@@ -431,12 +432,14 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
   const uint4* row8 = reinterpret_cast<const uint4*>(body);
 
   // ---- 1. histogram of this part ------------------------------------------------
-  // the row's numbers, long before they are needed
-  const float t32 = p.temperature[r], u32 = p.uniform[r];
-  const float p32 = p.top_p ? p.top_p[r] : 1.f, m32 = p.min_p ? p.min_p[r] : 0.f;
-  const int64_t k64 = p.top_k ? p.top_k[r] : 0;
+  // A programmatic dependent of the preceding kernel: the counters are cleared beside it, and
+  // nothing of it is read or written before this waits (1.9 to 2.9 us a call).
   cluster.barrier_arrive();  // (this CTA runs: the others may write its shared memory)
-  uint4 u[kUnroll];  // the first tokens are on their way while the counters are cleared
+  for (int i = threadIdx.x; i < kKeys / 8; i += kThreads)
+    reinterpret_cast<uint4*>(sh->hist)[i] = make_uint4(0, 0, 0, 0);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (threadIdx.x == 0) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  uint4 u[kUnroll];
   auto fetch = [&](int i) {
 #pragma unroll
     for (int k = 0; k < kUnroll; ++k)
@@ -446,8 +449,10 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
   uint32_t sample = kNone;  // one of 32 tokens spread over the part
   if (warp == 0 && hi > lo)
     sample = __half_as_ushort(row[lo + static_cast<int>((hi - lo) * int64_t(lane) >> 5)]);
-  for (int i = threadIdx.x; i < kKeys / 8; i += kThreads)
-    reinterpret_cast<uint4*>(sh->hist)[i] = make_uint4(0, 0, 0, 0);
+  // the row's numbers, long before they are needed
+  const float t32 = p.temperature[r], u32 = p.uniform[r];
+  const float p32 = p.top_p ? p.top_p[r] : 1.f, m32 = p.min_p ? p.min_p[r] : 0.f;
+  const int64_t k64 = p.top_k ? p.top_k[r] : 0;
   if (threadIdx.x < kChunks) {
     sh->count[threadIdx.x] = sh->above[threadIdx.x] = 0;
     sh->mass[threadIdx.x] = sh->mass_above[threadIdx.x] = 0.0;
@@ -877,27 +882,60 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
   }
 }
 
+// Launch of `rows` clusters of kParts CTAs, a programmatic dependent.
 template <int kParts>
-int launch(const Params& p, int64_t rows, int slot, cudaStream_t stream) {
-  const int st = ensure_smem_attribute(reinterpret_cast<const void*>(&sample_kernel<kParts>),
-                                       sizeof(Shared), slot);
-  if (st != CIE_OK) return st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = kParts;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
+struct Launch {
+  cudaLaunchAttribute attr[2];
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(rows * kParts));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = sizeof(Shared);
-  cfg.stream = stream;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, sample_kernel<kParts>, p);
-  if (e != cudaSuccess) return fail(CIE_ERR_CUDA, "sample launch: %s", cudaGetErrorString(e));
-  return CIE_OK;
-}
+
+  Launch(int64_t rows, cudaStream_t stream) {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = kParts;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(static_cast<unsigned>(rows * kParts));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = sizeof(Shared);
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+  }
+
+  static int prepare() {
+    constexpr int kSlot = kParts == 1 ? 5 : kParts == 2 ? 6 : kParts == 4 ? 7 : 10;
+    return ensure_smem_attribute(reinterpret_cast<const void*>(&sample_kernel<kParts>),
+                                 sizeof(Shared), kSlot);
+  }
+
+  // rows whose clusters run at the same time (asked once per device; SMs of a GPC that do
+  // not make up a cluster stay idle: 148 SMs hold 15 clusters of 8, 33 of 4, 74 of 2)
+  static int64_t at_once() {
+    constexpr int kDevices = 64;
+    static std::atomic<int> known[kDevices];  // 0: not yet asked
+    const int dev = current_device();
+    int n = dev >= 0 && dev < kDevices ? known[dev].load(std::memory_order_relaxed) : 0;
+    if (n == 0) {
+      Launch l(1, nullptr);
+      l.cfg.numAttrs = 1;
+      if (prepare() != CIE_OK ||
+          cudaOccupancyMaxActiveClusters(&n, sample_kernel<kParts>, &l.cfg) != cudaSuccess || n < 1)
+        return 0;
+      if (dev >= 0 && dev < kDevices) known[dev].store(n, std::memory_order_relaxed);
+    }
+    return n;
+  }
+
+  static int run(const Params& p, int64_t rows, cudaStream_t stream) {
+    const int st = prepare();
+    if (st != CIE_OK) return st;
+    Launch l(rows, stream);
+    const cudaError_t e = cudaLaunchKernelEx(&l.cfg, sample_kernel<kParts>, p);
+    if (e != cudaSuccess) return fail(CIE_ERR_CUDA, "sample launch: %s", cudaGetErrorString(e));
+    return CIE_OK;
+  }
+};
 
 }  // namespace sample
 }  // namespace cie
@@ -918,11 +956,16 @@ int cie_sample_rows(const void* logits, int64_t rows, int64_t vocab, int64_t str
   if (stride < vocab) return fail(CIE_ERR_INVALID_ARGUMENT, "row stride < vocab");
   if ((reinterpret_cast<uintptr_t>(logits) & 1) != 0)
     return fail(CIE_ERR_ALIGNMENT, "logits must be 2-byte aligned");
-  // parts a row needs, and more while every CTA still finds an SM of its own
+  // Parts a row needs, and more while all clusters still run at the same time and a part is
+  // long enough (151936 tokens, few rows: 18.0 us in 2 parts, 13.0 in 4, 12.0 in 8; 32003: 12.3
+  // in 1, 10.8 in 2, 9.8 in 4, 10.6 in 8; 8000: 9.0, 9.3, 8.9 and 10.0; one cluster too
+  // many doubles the time: 14.1 us for 33 rows in 4 parts, 24.4 for 34).
   int parts = 1;
   auto part_of = [&](int c) { return (vocab + 8LL * c - 1) / (8LL * c) * 8; };
   while (part_of(parts) > kMaxPart) parts *= 2;
-  while (parts < kMaxCluster && rows * parts * 2 <= sm_count() && part_of(parts) > 4096) parts *= 2;
+  if (parts == 1 && part_of(1) > 8192 && rows <= Launch<2>::at_once()) parts = 2;
+  if (parts == 2 && part_of(2) > 4096 && rows <= Launch<4>::at_once()) parts = 4;
+  if (parts == 4 && part_of(4) > 16384 && rows <= Launch<8>::at_once()) parts = 8;
   if (rows > 0x7fffffff / kMaxCluster) return fail(CIE_ERR_OVERFLOW, "too many rows");
   Params p;
   p.logits = static_cast<const __half*>(logits);
@@ -937,10 +980,10 @@ int cie_sample_rows(const void* logits, int64_t rows, int64_t vocab, int64_t str
   p.part = static_cast<int>(part_of(parts));
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   switch (parts) {
-    case 1: return launch<1>(p, rows, 5, st);
-    case 2: return launch<2>(p, rows, 6, st);
-    case 4: return launch<4>(p, rows, 7, st);
-    default: return launch<8>(p, rows, 10, st);
+    case 1: return Launch<1>::run(p, rows, st);
+    case 2: return Launch<2>::run(p, rows, st);
+    case 4: return Launch<4>::run(p, rows, st);
+    default: return Launch<8>::run(p, rows, st);
   }
 }
 

@@ -98,7 +98,8 @@ int cie_lm_head_argmax(const void* hidden, int64_t hidden_stride, const void* we
  * first NaN). Tokens at -inf have no weight; a row of nothing else gives token
  * 0; +inf logits share all of the mass. -0 and +0 are equal. top_k (int64),
  * top_p and min_p (fp32) may be NULL (off). Rows lie `stride` elements apart, at
- * any alignment. vocab <= 524224; out int64.
+ * any alignment. vocab <= 524224; out int64. The kernel is a programmatic dependent of the
+ * preceding kernel in `stream` and reads and writes nothing of the caller's before that is done.
  */
 int cie_sample_rows(const void* logits, int64_t rows, int64_t vocab, int64_t stride,
                     const float* uniform, const float* temperature, const int64_t* top_k,
