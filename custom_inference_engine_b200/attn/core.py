@@ -39,6 +39,7 @@ rope_kv_decode_attention_op = torch.ops.inference.rope_kv_decode_attention.defau
 rope_kv_mixed_attention_op = torch.ops.inference.rope_kv_mixed_attention.default
 rope_kv_q8_decode_update_op = torch.ops.inference.rope_kv_q8_decode_update.default
 rope_kv_q8_mixed_update_op = torch.ops.inference.rope_kv_q8_mixed_update.default
+rope_kv_q8_decode_attention_op = torch.ops.inference.rope_kv_q8_decode_attention.default
 gqa_decode_attention_q8_op = torch.ops.inference.gqa_decode_attention_q8.default
 _gqa_decode_attention_splits = torch.ops.inference.gqa_decode_attention_splits.default
 
@@ -117,9 +118,10 @@ class TritonQwen2Attention(torch.nn.Module):
     reference's modules never sets it, because the reference's piecewise
     backend splits the graph at ``inference::gqa_mixed_attention`` nodes
     (piecewise/utils.py:5-23), which the one-call form does not contain.
-    Over a ``QuantizedKVStorage`` both passes rotate, quantise and write in one
-    launch; a decode pass then attends to the 8-bit pages, a mixed pass reads its
-    histories back to fp16 pages and runs the mixed attention op on those.
+    Over a ``QuantizedKVStorage`` a decode pass is one call too
+    (``inference::rope_kv_q8_decode_attention``); a mixed pass rotates, quantises
+    and writes in one launch, reads its histories back to fp16 pages and runs the
+    mixed attention op on those.
     Without ``kv_manager`` it defers to the wrapped HF module.
     """
 
@@ -226,6 +228,8 @@ class TritonQwen2Attention(torch.nn.Module):
         slots, table = metadata.slot_ids, kv.block_table
         lens = getattr(metadata, "attn_lens", None)
         if metadata.full_decode:
+            if self.fuse_rope and self.fuse_decode_attention:
+                return rope_kv_q8_decode_attention_op(qkv, cos, sin, *pool, kv.lens, slots, table)
             if lens is None:
                 lens = kv.lens[slots] + 1
             if self.fuse_rope:

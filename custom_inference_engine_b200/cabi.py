@@ -325,6 +325,29 @@ def decode_attention_q8(q, k, v, kv_scales, lens, slot_ids, block_table, out=Non
     return out
 
 
+def rope_kv_q8_decode_attention(qkv, cos, sin, k_cache, v_cache, kv_scales, lens, slot_ids,
+                                block_table, num_splits: int = 0,
+                                workspace: Optional[torch.Tensor] = None,
+                                stream=None) -> torch.Tensor:
+    """cie_rope_kv_q8_decode_attention: ``lens`` per slot, before the new row."""
+    B, hkv, d = slot_ids.shape[0], k_cache.shape[1], k_cache.shape[3]
+    hq = qkv.shape[2] // d - 2 * hkv
+    S = num_splits if num_splits > 0 else decode_q8_default_splits(B, qkv.device.index or 0)
+    out = torch.empty((1, B, hq, d), dtype=qkv.dtype, device=qkv.device)
+    if workspace is None:
+        need = int(native.lib().cie_rope_kv_q8_decode_workspace_bytes(B, hq, d, S))
+        workspace = torch.empty(need, dtype=torch.uint8, device=qkv.device)
+    st = _entry("cie_rope_kv_q8_decode_attention", block_table)(
+        _p(qkv), qkv.stride(1), _p(cos), _p(sin), cos.stride(1),
+        *_q8_pool(k_cache, v_cache, kv_scales), _p(lens), _p(slot_ids), _p(block_table), _p(out),
+        _p(workspace), workspace.numel() * workspace.element_size(), B, hq, hkv, d,
+        k_cache.shape[2],
+        *_q8_strides(k_cache, min(lens.shape[0], block_table.shape[0]), block_table), S,
+        native.stream_ptr(stream))
+    native.check(st, "cie_rope_kv_q8_decode_attention")
+    return out
+
+
 def sample_rows(logits, uniform, temperature, top_k=None, top_p=None, min_p=None, out=None,
                 stream=None) -> torch.Tensor:
     """cie_sample_rows: a token per row of (rows, vocab) fp16 logits."""

@@ -24,7 +24,7 @@ EncodeTiledFn g_encode = nullptr;
 std::once_flag g_encode_once;
 cudaError_t g_encode_err = cudaSuccess;
 
-constexpr int kMaxSmemSlots = 16;
+constexpr int kMaxSmemSlots = 20;
 bool g_smem_set[kMaxDevices][kMaxSmemSlots] = {};
 std::mutex g_smem_mu;
 }  // namespace

@@ -68,7 +68,7 @@ struct Params {
   const int8_t* k;          // (n_pages, HKV, 16, 64)
   const int8_t* v;
   const float* scales;      // (n_pages, 2, HKV)
-  const int64_t* lens;      // (B,)
+  const int64_t* lens;      // (B,) keys; after an update of the call (n_slots,) without the new row
   const int64_t* slot_ids;  // (B,)
   BlockTable table;         // (n_slots, bt_stride)
   __half* o;                // (B, H_q, D)
@@ -76,6 +76,7 @@ struct Params {
   float* ws_ml;             // (B, S, H_q, 2)
   int num_splits;
   int group;                // query heads per kv head, 1..8
+  int after_update;         // q and each row's last page are the preceding kernel's
   int64_t n_pages, n_slots, bt_stride;
   int64_t page_stride, head_stride;
 };
@@ -125,10 +126,16 @@ __device__ __forceinline__ uint32_t codes_to_half2(uint32_t w, uint32_t sel, uin
 }
 
 __device__ __forceinline__ int seq_pages(const Params& p, int b) {
-  return decode::seq_pages(p.lens, p.slot_ids, b, p.n_slots, p.bt_stride, 0);
+  return decode::seq_pages(p.lens, p.slot_ids, b, p.n_slots, p.bt_stride, p.after_update);
 }
 
-template <int HKV>
+// kAfterUpdate: the preceding kernel is the same call's update, which writes q and, of
+// every row's pages, the last one, with its scale. It has itself waited for everything before
+// it when this grid starts, so that a warp's first pages are fetched while it runs (64 rows
+// of 650 keys: 12.7 us for the call, 15.1 us as two calls; 256 of 2000: 42.2 and 46.3).
+// Rotating q here as well and waiting only before the last page is read won 0.7 to 1.5 us at
+// 64 rows and lost 1.4 to 2.2 us at 256 (registers let one CTA of two start beside the update).
+template <int HKV, bool kAfterUpdate>
 __global__ void __launch_bounds__(32 * kWarps, 2) decode_q8_split_kernel(const Params p) {
   using C = Cfg<HKV>;
   constexpr int kHeads = C::kHeads, kStep = C::kStep, kRing = C::kRing, kThreads = 32 * kWarps;
@@ -149,15 +156,21 @@ __global__ void __launch_bounds__(32 * kWarps, 2) decode_q8_split_kernel(const P
     fence_mbar_init();
   }
   __syncwarp();
-  // a programmatic dependent of the preceding kernel: no input is read before this
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (threadIdx.x == 0) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  // a programmatic dependent of the preceding kernel: nothing that it writes is read before
+  auto wait = [] {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (threadIdx.x == 0) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  };
+  if (!kAfterUpdate) wait();
 
-  const int64_t slot = p.slot_ids[b];
-  int64_t L = p.lens[b];
+  // what is read before the wait comes from L2: this SM's L1 may hold older lines
+  auto load = [](const auto* x) { return kAfterUpdate ? __ldcg(x) : *x; };
+  const int64_t slot = load(p.slot_ids + b);
+  int64_t L = 0;
   if (slot < 0 || slot >= p.n_slots) {
     if (threadIdx.x == 0) raise_error(CIE_DEVERR_BAD_SLOT);
-    L = 0;
+  } else {
+    L = kAfterUpdate ? load(p.lens + slot) + 1 : load(p.lens + b);
   }
   if (L < 0) L = 0;
   if ((L + kPage - 1) / kPage > p.bt_stride) {
@@ -175,7 +188,10 @@ __global__ void __launch_bounds__(32 * kWarps, 2) decode_q8_split_kernel(const P
   // entries of the next 32 on their way). Scales: ks times head_dim ** -0.5 * log2(e).
   const int64_t bt_row = slot * p.bt_stride + page_begin + par;
   auto entry = [&](int i) -> int64_t {
-    return i < mine ? p.table.at(bt_row + static_cast<int64_t>(i) * kStep) : 0;
+    const int64_t at = bt_row + static_cast<int64_t>(i) * kStep;
+    if (i >= mine) return 0;
+    return p.table.wide ? load(static_cast<const int64_t*>(p.table.ptr) + at)
+                        : load(static_cast<const int32_t*>(p.table.ptr) + at);
   };
   int64_t entry_n = entry(lane);
   int pid = 0;
@@ -211,14 +227,31 @@ __global__ void __launch_bounds__(32 * kWarps, 2) decode_q8_split_kernel(const P
       const float* sp = p.scales + static_cast<int64_t>(pid) * (2 * HKV) + h0;
 #pragma unroll
       for (int u = 0; u < kHeads; ++u) {
-        ks_n[u] = sp[u] * (0.125f * kLog2e);
-        vs_n[u] = sp[HKV + u];
+        ks_n[u] = load(sp + u) * (0.125f * kLog2e);
+        vs_n[u] = load(sp + HKV + u);
       }
       entry_n = entry(i + 32 + lane);
     }
   };
+  int ahead = 0;  // pages fetched before the update is done
+  if (kAfterUpdate) {
+    // among this warp's pages the row's last one is number `last`, if it is there at all
+    const int behind = n_seq_pages - 1 - (page_begin + par);
+    const int last = behind % kStep == 0 ? behind / kStep : mine;
 #pragma unroll 1
-  for (int u = 0; u < kRing; ++u) fetch(u);
+    for (; ahead < min(kRing, last); ++ahead) fetch(ahead);
+    wait();
+    if (ahead > 0 && lane == last && last < mine) {  // its scale was read with the first 32
+      const float* sp = p.scales + static_cast<int64_t>(pid) * (2 * HKV) + h0;
+#pragma unroll
+      for (int u = 0; u < kHeads; ++u) {
+        ks_n[u] = __ldcg(sp + u) * (0.125f * kLog2e);
+        vs_n[u] = __ldcg(sp + HKV + u);
+      }
+    }
+  }
+#pragma unroll 1
+  for (int u = ahead; u < kRing; ++u) fetch(u);
 
   uint32_t bq[kHeads][4][2];
   float m[kHeads][2], l[kHeads][2];  // query heads 2 t, 2 t + 1 of each kv head; m in log2
@@ -487,10 +520,11 @@ __global__ void __launch_bounds__(kFold > 1 ? 32 * kFold : 1024) merge_q8_kernel
       __floats2half2_rn(acc.x * inv, acc.y * inv);
 }
 
-template <int HKV>
+template <int HKV, bool kAfterUpdate>
 int launch(const Params& p, int batch, cudaStream_t stream) {
-  const int st = ensure_smem_attribute(reinterpret_cast<const void*>(&decode_q8_split_kernel<HKV>),
-                                       Cfg<HKV>::kSmemBytes, 10 + HKV);
+  const auto split_kernel = decode_q8_split_kernel<HKV, kAfterUpdate>;
+  const int st = ensure_smem_attribute(reinterpret_cast<const void*>(split_kernel),
+                                       Cfg<HKV>::kSmemBytes, (kAfterUpdate ? 14 : 10) + HKV);
   if (st != CIE_OK) return st;
   cudaLaunchAttribute pdl[1];
   pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -502,7 +536,7 @@ int launch(const Params& p, int batch, cudaStream_t stream) {
   cfg.stream = stream;
   cfg.attrs = pdl;
   cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, decode_q8_split_kernel<HKV>, p);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, split_kernel, p);
   if (e != cudaSuccess) return fail(CIE_ERR_CUDA, "decode_q8 launch: %s", cudaGetErrorString(e));
   if (p.num_splits > 1) {
     const int H_Q = HKV * p.group;
@@ -517,13 +551,13 @@ int launch(const Params& p, int batch, cudaStream_t stream) {
   return CIE_OK;
 }
 
-int entry(const void* q, const void* k, const void* v, const float* kv_scales,
-          const int64_t* lens, const int64_t* slot_ids, BlockTable table, void* o,
-          void* workspace, size_t workspace_bytes, int batch, int num_q_heads, int num_kv_heads,
-          int head_dim, int page_size, int64_t n_pages, int64_t n_slots, int64_t bt_stride,
-          int64_t page_stride, int64_t head_stride, int num_splits, cie_stream_t stream) {
-  if (batch < 0) return fail(CIE_ERR_INVALID_ARGUMENT, "batch < 0");
-  if (batch == 0) return CIE_OK;
+// Checks of a call; sets what is common to both entry points. `q_bytes` of the workspace
+// lie in front of the partials.
+int prepare(Params& p, const void* q, const void* k, const void* v, const float* kv_scales,
+            const int64_t* lens, const int64_t* slot_ids, BlockTable table, void* o,
+            void* workspace, size_t workspace_bytes, size_t q_bytes, int batch, int num_q_heads,
+            int num_kv_heads, int head_dim, int page_size, int64_t n_pages, int64_t n_slots,
+            int64_t bt_stride, int64_t page_stride, int64_t head_stride, int num_splits) {
   if (!q || !lens || !slot_ids || !table.ptr || !o)
     return fail(CIE_ERR_INVALID_ARGUMENT, "null pointer argument");
   const int st = kvq8::check_pool(k, v, kv_scales, num_kv_heads, head_dim, page_size, n_pages,
@@ -542,14 +576,14 @@ int entry(const void* q, const void* k, const void* v, const float* kv_scales,
   if (!aligned16(q) || !aligned16(o)) return fail(CIE_ERR_ALIGNMENT, "q / o must be 16-byte aligned");
   const int S = num_splits > 0 ? num_splits : cie_decode_q8_default_splits(batch, current_device());
   if (S > 4096) return fail(CIE_ERR_INVALID_ARGUMENT, "num_splits %d > 4096", S);
-  Params p{};
-  if (S > 1) {
-    const size_t need = cie_decode_workspace_bytes(batch, num_q_heads, head_dim, S);
+  const size_t need =
+      q_bytes + (S > 1 ? cie_decode_workspace_bytes(batch, num_q_heads, head_dim, S) : 0);
+  if (need > 0) {
     if (workspace == nullptr || workspace_bytes < need)
-      return fail(CIE_ERR_WORKSPACE, "split path needs %zu workspace bytes, got %zu", need,
+      return fail(CIE_ERR_WORKSPACE, "the call needs %zu workspace bytes, got %zu", need,
                   workspace == nullptr ? size_t(0) : workspace_bytes);
     if (!aligned16(workspace)) return fail(CIE_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
-    p.ws_acc = static_cast<float*>(workspace);
+    p.ws_acc = reinterpret_cast<float*>(static_cast<char*>(workspace) + q_bytes);
     p.ws_ml = p.ws_acc + static_cast<int64_t>(batch) * S * num_q_heads * kD;
   }
   p.q = static_cast<const __half*>(q);
@@ -567,12 +601,62 @@ int entry(const void* q, const void* k, const void* v, const float* kv_scales,
   p.bt_stride = bt_stride;
   p.page_stride = page_stride;
   p.head_stride = head_stride;
+  return CIE_OK;
+}
+
+template <bool kAfterUpdate>
+int run(const Params& p, int batch, int num_kv_heads, cie_stream_t stream) {
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   switch (num_kv_heads) {
-    case 1: return launch<1>(p, batch, s);
-    case 2: return launch<2>(p, batch, s);
-    default: return launch<4>(p, batch, s);
+    case 1: return launch<1, kAfterUpdate>(p, batch, s);
+    case 2: return launch<2, kAfterUpdate>(p, batch, s);
+    default: return launch<4, kAfterUpdate>(p, batch, s);
   }
+}
+
+int entry(const void* q, const void* k, const void* v, const float* kv_scales,
+          const int64_t* lens, const int64_t* slot_ids, BlockTable table, void* o,
+          void* workspace, size_t workspace_bytes, int batch, int num_q_heads, int num_kv_heads,
+          int head_dim, int page_size, int64_t n_pages, int64_t n_slots, int64_t bt_stride,
+          int64_t page_stride, int64_t head_stride, int num_splits, cie_stream_t stream) {
+  if (batch < 0) return fail(CIE_ERR_INVALID_ARGUMENT, "batch < 0");
+  if (batch == 0) return CIE_OK;
+  Params p{};
+  const int st = prepare(p, q, k, v, kv_scales, lens, slot_ids, table, o, workspace,
+                         workspace_bytes, 0, batch, num_q_heads, num_kv_heads, head_dim,
+                         page_size, n_pages, n_slots, bt_stride, page_stride, head_stride,
+                         num_splits);
+  return st != CIE_OK ? st : run<false>(p, batch, num_kv_heads, stream);
+}
+
+// Rotated q in front of the split scratch.
+size_t q_bytes(int batch, int num_q_heads, int head_dim) {
+  return static_cast<size_t>(batch) * num_q_heads * head_dim * sizeof(__half);
+}
+
+int rope_entry(const void* qkv, int64_t qkv_tok, const void* cos, const void* sin,
+               int64_t cs_tok, void* k, void* v, float* kv_scales, const int64_t* lens,
+               const int64_t* slot_ids, BlockTable table, void* o, void* workspace,
+               size_t workspace_bytes, int batch, int num_q_heads, int num_kv_heads,
+               int head_dim, int page_size, int64_t n_pages, int64_t n_slots, int64_t bt_stride,
+               int64_t page_stride, int64_t head_stride, int num_splits, cie_stream_t stream) {
+  if (batch < 0) return fail(CIE_ERR_INVALID_ARGUMENT, "batch < 0");
+  if (batch == 0) return CIE_OK;
+  if (!workspace) return fail(CIE_ERR_WORKSPACE, "no workspace");
+  Params p{};
+  int st = prepare(p, workspace, k, v, kv_scales, lens, slot_ids, table, o, workspace,
+                   workspace_bytes, q_bytes(batch, num_q_heads, kD), batch, num_q_heads,
+                   num_kv_heads, head_dim, page_size, n_pages, n_slots, bt_stride, page_stride,
+                   head_stride, num_splits);
+  if (st != CIE_OK) return st;
+  p.after_update = 1;
+  kvq8::Args a = kvq8::pool_args(k, v, kv_scales, slot_ids, table, batch, num_kv_heads, n_pages,
+                                 n_slots, bt_stride, page_stride, head_stride);
+  kvq8::set_rope(a, qkv, qkv_tok, cos, sin, cs_tok, workspace, num_q_heads);
+  a.lens = lens;
+  a.tokens = batch;
+  st = kvq8::update(a, true, false, head_dim, page_size, stream);
+  return st != CIE_OK ? st : run<true>(p, batch, num_kv_heads, stream);
 }
 
 }  // namespace dq8
@@ -625,6 +709,41 @@ int cie_decode_attention_q8_bt32(const void* q, const void* k, const void* v,
                          workspace, workspace_bytes, batch, num_q_heads, num_kv_heads, head_dim,
                          page_size, n_pages, n_slots, bt_stride, kv_page_stride, kv_head_stride,
                          num_splits, stream);
+}
+
+size_t cie_rope_kv_q8_decode_workspace_bytes(int batch, int num_q_heads, int head_dim,
+                                             int num_splits) {
+  if (batch <= 0 || num_q_heads <= 0 || head_dim <= 0) return 0;
+  return cie::dq8::q_bytes(batch, num_q_heads, head_dim) +
+         (num_splits > 1 ? cie_decode_workspace_bytes(batch, num_q_heads, head_dim, num_splits) : 0);
+}
+
+int cie_rope_kv_q8_decode_attention(
+    const void* qkv, int64_t qkv_tok_stride, const void* cos, const void* sin,
+    int64_t cs_tok_stride, void* k_cache, void* v_cache, float* kv_scales, const int64_t* lens,
+    const int64_t* slot_ids, const int64_t* block_table, void* o, void* workspace,
+    size_t workspace_bytes, int batch, int num_q_heads, int num_kv_heads, int head_dim,
+    int page_size, int64_t n_pages, int64_t n_slots, int64_t bt_stride,
+    int64_t cache_page_stride, int64_t cache_head_stride, int num_splits, cie_stream_t stream) {
+  return cie::dq8::rope_entry(qkv, qkv_tok_stride, cos, sin, cs_tok_stride, k_cache, v_cache,
+                              kv_scales, lens, slot_ids, cie::BlockTable{block_table, 1}, o,
+                              workspace, workspace_bytes, batch, num_q_heads, num_kv_heads,
+                              head_dim, page_size, n_pages, n_slots, bt_stride,
+                              cache_page_stride, cache_head_stride, num_splits, stream);
+}
+
+int cie_rope_kv_q8_decode_attention_bt32(
+    const void* qkv, int64_t qkv_tok_stride, const void* cos, const void* sin,
+    int64_t cs_tok_stride, void* k_cache, void* v_cache, float* kv_scales, const int64_t* lens,
+    const int64_t* slot_ids, const int32_t* block_table, void* o, void* workspace,
+    size_t workspace_bytes, int batch, int num_q_heads, int num_kv_heads, int head_dim,
+    int page_size, int64_t n_pages, int64_t n_slots, int64_t bt_stride,
+    int64_t cache_page_stride, int64_t cache_head_stride, int num_splits, cie_stream_t stream) {
+  return cie::dq8::rope_entry(qkv, qkv_tok_stride, cos, sin, cs_tok_stride, k_cache, v_cache,
+                              kv_scales, lens, slot_ids, cie::BlockTable{block_table, 0}, o,
+                              workspace, workspace_bytes, batch, num_q_heads, num_kv_heads,
+                              head_dim, page_size, n_pages, n_slots, bt_stride,
+                              cache_page_stride, cache_head_stride, num_splits, stream);
 }
 
 }  // extern "C"

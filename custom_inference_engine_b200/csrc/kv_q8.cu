@@ -62,7 +62,7 @@ __device__ __forceinline__ void start_as_dependent() {
 
 __device__ __forceinline__ void load8(const __half* p, int vec, float (&x)[8]) {
   if (vec) {
-    const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
     const __half2* h = reinterpret_cast<const __half2*>(&u);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {

@@ -569,6 +569,40 @@ at::Tensor rope_kv_q8_decode_update(const at::Tensor& qkv, const at::Tensor& cos
   return q;
 }
 
+at::Tensor rope_kv_q8_decode_attention(const at::Tensor& qkv, const at::Tensor& cos,
+                                       const at::Tensor& sin, at::Tensor& k_cache,
+                                       at::Tensor& v_cache, at::Tensor& kv_scales,
+                                       const at::Tensor& lens, const at::Tensor& slot_ids,
+                                       const at::Tensor& block_table) {
+  check_q8_pool(k_cache, v_cache, kv_scales);
+  check_q8_rope(qkv, cos, sin, k_cache);
+  check_q8_tables(k_cache, slot_ids, block_table);
+  check_slot_lens(lens, k_cache);
+  TORCH_CHECK(slot_ids.size(0) == qkv.size(1), "one token per slot id");
+  c10::cuda::CUDAGuard guard(qkv.device());
+  at::Tensor o = rope_out(qkv, k_cache);
+  const int B = static_cast<int>(slot_ids.size(0)), hq = static_cast<int>(o.size(2)),
+            d = static_cast<int>(o.size(3));
+  if (B == 0) return o;
+  const int S = cie_decode_q8_default_splits(B, qkv.get_device());
+  const size_t ws_bytes = cie_rope_kv_q8_decode_workspace_bytes(B, hq, d, S);
+  at::Tensor ws = at::empty({static_cast<int64_t>(ws_bytes)}, qkv.options().dtype(at::kByte));
+  const int st = with_table(
+      block_table,
+      [&](auto fn, auto* table) {
+        return fn(qkv.data_ptr(), qkv.stride(1), cos.data_ptr(), sin.data_ptr(), cos.stride(1),
+                  k_cache.data_ptr(), v_cache.data_ptr(), kv_scales.data_ptr<float>(),
+                  lens.data_ptr<int64_t>(), slot_ids.data_ptr<int64_t>(), table, o.data_ptr(),
+                  ws.data_ptr(), ws_bytes, B, hq, static_cast<int>(k_cache.size(1)), d,
+                  static_cast<int>(k_cache.size(2)), k_cache.size(0), slots_of(lens, block_table),
+                  block_table.stride(0), k_cache.stride(0), k_cache.stride(1), S,
+                  current_stream());
+      },
+      cie_rope_kv_q8_decode_attention, cie_rope_kv_q8_decode_attention_bt32);
+  check_status(st, "rope_kv_q8_decode_attention");
+  return o;
+}
+
 at::Tensor rope_kv_q8_mixed_update(const at::Tensor& qkv, const at::Tensor& cos,
                                    const at::Tensor& sin, at::Tensor& k_cache,
                                    at::Tensor& v_cache, at::Tensor& kv_scales,
@@ -849,6 +883,10 @@ TORCH_LIBRARY(inference, m) {
       "Tensor(b!) v_cache, Tensor(c!) kv_scales, Tensor lens, Tensor slot_ids, "
       "Tensor block_table) -> Tensor");
   m.def(
+      "rope_kv_q8_decode_attention(Tensor qkv, Tensor cos, Tensor sin, Tensor(a!) k_cache, "
+      "Tensor(b!) v_cache, Tensor(c!) kv_scales, Tensor lens, Tensor slot_ids, "
+      "Tensor block_table) -> Tensor");
+  m.def(
       "rope_kv_q8_mixed_update(Tensor qkv, Tensor cos, Tensor sin, Tensor(a!) k_cache, "
       "Tensor(b!) v_cache, Tensor(c!) kv_scales, Tensor cu_seqlens, Tensor kv_lens, "
       "Tensor slot_ids, Tensor block_table) -> Tensor");
@@ -886,6 +924,7 @@ TORCH_LIBRARY_IMPL(inference, CUDA, m) {
   m.impl("kv_q8_decode_update", &kv_q8_decode_update);
   m.impl("kv_q8_mixed_update", &kv_q8_mixed_update);
   m.impl("rope_kv_q8_decode_update", &rope_kv_q8_decode_update);
+  m.impl("rope_kv_q8_decode_attention", &rope_kv_q8_decode_attention);
   m.impl("rope_kv_q8_mixed_update", &rope_kv_q8_mixed_update);
   m.impl("kv_q8_read", &kv_q8_read);
   m.impl("gqa_decode_attention_q8", &gqa_decode_attention_q8);

@@ -83,13 +83,16 @@ SIGNATURES.update({
     "cie_decode_q8_default_splits": (c_int, [c_int, c_int]),
     "cie_decode_attention_q8": (c_int, [c_ptr] * 9 + [c_size] + [c_int] * 5 + [c_i64] * 5
                                 + [c_int, c_ptr]),
+    "cie_rope_kv_q8_decode_workspace_bytes": (c_size, [c_int] * 4),
+    "cie_rope_kv_q8_decode_attention": (c_int, [c_ptr, c_i64, c_ptr, c_ptr, c_i64] + [c_ptr] * 8
+                                        + [c_size] + [c_int] * 5 + [c_i64] * 5 + [c_int, c_ptr]),
 })
 # the int32-block-table variants take the same arguments
 for _name in ("cie_decode_attention", "cie_mixed_attention", "cie_kv_decode_update",
               "cie_rope_kv_decode_update", "cie_rope_kv_decode_attention",
               "cie_rope_kv_mixed_attention", "cie_kv_q8_decode_update", "cie_kv_q8_mixed_update",
               "cie_rope_kv_q8_decode_update", "cie_rope_kv_q8_mixed_update", "cie_kv_q8_read",
-              "cie_decode_attention_q8"):
+              "cie_decode_attention_q8", "cie_rope_kv_q8_decode_attention"):
     SIGNATURES[_name + "_bt32"] = SIGNATURES[_name]
 SIGNATURES.update({
     # include/cie_model_ops.h
@@ -246,6 +249,11 @@ def _register_fakes() -> None:
     @torch.library.register_fake("inference::rope_kv_q8_mixed_update")
     def _rope_q8_mix_fake(qkv, cos, sin, k_cache, v_cache, kv_scales, cu_seqlens, kv_lens,
                           slot_ids, block_table):
+        return _rope_out(qkv, k_cache)
+
+    @torch.library.register_fake("inference::rope_kv_q8_decode_attention")
+    def _rope_q8_dec_attn_fake(qkv, cos, sin, k_cache, v_cache, kv_scales, lens, slot_ids,
+                               block_table):
         return _rope_out(qkv, k_cache)
 
     @torch.library.register_fake("inference::kv_q8_read")

@@ -202,6 +202,33 @@ int cie_decode_attention_q8_bt32(const void* q, const void* k, const void* v,
                                  int64_t kv_page_stride, int64_t kv_head_stride, int num_splits,
                                  cie_stream_t stream);
 
+/*
+ * The attention step of a decode pass in one call (cie_rope_kv_decode_attention over
+ * the 8-bit pool): cie_rope_kv_q8_decode_update, then cie_decode_attention_q8 over the
+ * lens[s] + 1 rows of every sequence's slot s, bit for bit; `lens` is per slot, the
+ * length before the new row, and is not advanced. The attention starts while the
+ * update runs: a page that the call writes must be the last page of every sequence
+ * that reads it (of padding rows that share one page the result is unspecified).
+ * `workspace`: cie_rope_kv_q8_decode_workspace_bytes(batch, num_q_heads,
+ * head_dim, splits) bytes, 16-byte aligned, for the rotated q and the splits.
+ */
+size_t cie_rope_kv_q8_decode_workspace_bytes(int batch, int num_q_heads, int head_dim,
+                                             int num_splits);
+int cie_rope_kv_q8_decode_attention(
+    const void* qkv, int64_t qkv_tok_stride, const void* cos, const void* sin,
+    int64_t cs_tok_stride, void* k_cache, void* v_cache, float* kv_scales, const int64_t* lens,
+    const int64_t* slot_ids, const int64_t* block_table, void* o, void* workspace,
+    size_t workspace_bytes, int batch, int num_q_heads, int num_kv_heads, int head_dim,
+    int page_size, int64_t n_pages, int64_t n_slots, int64_t bt_stride,
+    int64_t cache_page_stride, int64_t cache_head_stride, int num_splits, cie_stream_t stream);
+int cie_rope_kv_q8_decode_attention_bt32(
+    const void* qkv, int64_t qkv_tok_stride, const void* cos, const void* sin,
+    int64_t cs_tok_stride, void* k_cache, void* v_cache, float* kv_scales, const int64_t* lens,
+    const int64_t* slot_ids, const int32_t* block_table, void* o, void* workspace,
+    size_t workspace_bytes, int batch, int num_q_heads, int num_kv_heads, int head_dim,
+    int page_size, int64_t n_pages, int64_t n_slots, int64_t bt_stride,
+    int64_t cache_page_stride, int64_t cache_head_stride, int num_splits, cie_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
