@@ -33,7 +33,7 @@
 // kernel.
 //
 // Measured (B200, cold pages): 256 x 4096 rows, two heads, 51 us = 5.3 TB/s, 0.81 of the
-// measured copy bandwidth; 64 x 16001-32768 80 us; one sequence of 511 rows 5.3 us, of
+// measured copy bandwidth; 64 x 16001-32768 80 us; one sequence of 511 rows 4.5 us, of
 // 16384 7.8 us. What bounds it: the pages' bandwidth at large sizes, with 16 warps per SM
 // (128 registers) and about 240 instructions a page and head; the chain slot -> length ->
 // block table -> page -> merge at small ones.
@@ -166,11 +166,12 @@ __global__ void __launch_bounds__(32 * kWarps, 2) decode_q8_split_kernel(const P
   // what is read before the wait comes from L2: this SM's L1 may hold older lines
   auto load = [](const auto* x) { return kAfterUpdate ? __ldcg(x) : *x; };
   const int64_t slot = load(p.slot_ids + b);
-  int64_t L = 0;
+  int64_t L = kAfterUpdate ? 0 : load(p.lens + b);  // (beside the slot)
   if (slot < 0 || slot >= p.n_slots) {
     if (threadIdx.x == 0) raise_error(CIE_DEVERR_BAD_SLOT);
-  } else {
-    L = kAfterUpdate ? load(p.lens + slot) + 1 : load(p.lens + b);
+    L = 0;
+  } else if (kAfterUpdate) {
+    L = load(p.lens + slot) + 1;
   }
   if (L < 0) L = 0;
   if ((L + kPage - 1) / kPage > p.bt_stride) {
