@@ -221,7 +221,6 @@ class TritonQwen2Attention(torch.nn.Module):
         out = self.original.o_proj(o.reshape(1, total_T, self.num_heads * self.head_dim))
         return out, None
 
-
     def _quantized_attention(self, qkv, cos, sin, kv, metadata):
         """Write and attention of one pass over 8-bit pages."""
         layer, pool = self.layer_idx, kv.pool(self.layer_idx)
