@@ -157,6 +157,46 @@ def test_layers_in_a_captured_step(ops, cuda_device):
             assert torch.equal(a, b)
 
 
+def test_two_streams_at_once(ops, cuda_device):
+    """Decode passes and sampled tokens of two models on streams of their own."""
+    dev, steps = cuda_device, 30
+    sides = []
+    for seed, hist in ((1, [700, 15, 3000, 31]), (2, [16, 900, 63, 2048, 5])):
+        (k, v, s, lens, bt), g = _case(hist, 2, 7, seed, dev, room=steps)
+        slots = torch.arange(1, len(hist) + 1, device=dev)
+        tokens = []
+        at = lens.clone()
+        for _ in range(steps):
+            tokens.append(_token(len(hist), 2, 7, at[slots], g, dev, big=2.0))
+            at[1:] += 1
+        logits = (torch.randn(len(hist), 60000, generator=g) * 3).half().to(dev)
+        u = torch.rand(steps, len(hist), generator=g).to(dev)
+        sides.append((k, v, s, lens, bt, slots, tokens, logits, u, torch.ones(len(hist), device=dev)))
+
+    def step(side, pools, at, i, op):
+        _, _, _, _, bt, slots, tokens, logits, u, t = side
+        return op(*tokens[i], *pools, at, slots, bt), ops.sample_rows(logits, u[i], t)
+
+    want = []
+    for side in sides:
+        pools, at = [x.clone() for x in side[:3]], side[3].clone()
+        for i in range(steps):
+            want.append(step(side, pools, at, i, lambda *a: _in_sequence(ops, *a)))
+            at[1:] += 1
+    streams = [torch.cuda.Stream() for _ in sides]
+    state = [([x.clone() for x in side[:3]], side[3].clone()) for side in sides]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for i in range(steps):
+        for n, (side, (pools, at), stream) in enumerate(zip(sides, state, streams)):
+            with torch.cuda.stream(stream):
+                got[n].append(step(side, pools, at, i, ops.rope_kv_q8_decode_attention))
+                at[1:] += 1
+    torch.cuda.synchronize()
+    for (a, b), (c, d) in zip(got[0] + got[1], want):
+        assert torch.equal(a, c) and torch.equal(b, d)
+
+
 def test_a_refused_call_writes_nothing(ops, cuda_device):
     dev = cuda_device
     (k, v, s, lens, bt), g = _case([20, 40], 2, 7, 1, dev)
