@@ -109,14 +109,17 @@ __device__ __forceinline__ uint4 ldg16(const __half* ptr) {
 constexpr int kMinPagesPerSplit = 4;
 
 // Pages of sequence b that the kernels visit; 0 for an invalid slot. A length
-// beyond the block-table row is clamped to it.
+// beyond the block-table row is clamped to it. Read past L1: the merge kernels
+// call this before they wait, when this SM's L1 may still hold lines from before
+// the kernel or copy that set the lengths, and a merge that cut a sequence
+// otherwise than the split kernel did would read partials that nobody wrote.
 __device__ __forceinline__ int seq_pages(const int64_t* lens, const int64_t* slot_ids, int b,
                                          int64_t n_slots, int64_t bt_stride, int lens_per_slot) {
-  const int64_t slot = slot_ids[b];
+  const int64_t slot = __ldcg(slot_ids + b);
   if (slot < 0 || slot >= n_slots) return 0;
   // per sequence: keys visible to the query; per slot: the slot's length
   // before the query token, which is then written and attended to as well
-  int64_t L = lens_per_slot ? lens[slot] + 1 : lens[b];
+  int64_t L = lens_per_slot ? __ldcg(lens + slot) + 1 : __ldcg(lens + b);
   if (L < 0) L = 0;
   const int64_t np = (L + kPage - 1) / kPage;
   return static_cast<int>(np > bt_stride ? bt_stride : np);

@@ -475,7 +475,7 @@ __global__ void __launch_bounds__(kFold > 1 ? 32 * kFold : 1024) merge_q8_kernel
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int H_Q = HKV * p.group;
   const int b = blockIdx.x, hq = kFold > 1 ? blockIdx.y : warp, fold = kFold > 1 ? warp : 0;
-  // (the split kernel does not write slots and lengths)
+  // (the split kernel does not write slots and lengths; read past L1)
   const int n = seq_pages(p, b);
   const int pps = decode::split_pages(n, p.num_splits);
   // Every CTA waits, also one with nothing to merge: a grid that ended without waiting

@@ -32,7 +32,10 @@
  * 0, and both set CIE_DEVERR_NONFINITE. Pages may be shared by slots that read
  * them; the sequences of one update call must write different pages.
  * The kernels are programmatic dependents of the preceding kernel in `stream` and
- * touch nothing before it is done.
+ * touch nothing of the caller's before it is done. Inside a call the later kernels start
+ * early: the merge of several splits reads slots and lengths beside the split
+ * kernel, and the attention of cie_rope_kv_q8_decode_attention reads slots, lengths, block
+ * table and older pages beside the update, none of which the earlier kernel writes.
  */
 #ifndef CIE_KV_Q8_H_
 #define CIE_KV_Q8_H_
