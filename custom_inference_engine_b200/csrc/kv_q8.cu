@@ -8,7 +8,8 @@
 // at most one final step off (half a step for the final rounding, and the halves
 // of all earlier steps together are less than another), where re-rounding to
 // arbitrary scales would add half a step for each growth. x / 2^e is exact in
-// fp32 and code * 2^e in fp16, so every code follows from the values alone.
+// fp32 and code * 2^e in fp16, so every code follows from the values alone. A page
+// that was filled elsewhere may come with any scale; it keeps it while new rows fit.
 //
 // All rows of a page that a call writes are quantised together, by one warp per
 // (page, K or V, kv head): lane l holds chunk l mod 8 (8 of the 64 values) of
@@ -91,12 +92,21 @@ __device__ __forceinline__ int need_exp(float amax) {
   return min(max(e, kMinExp), kMaxExp);
 }
 
-// The stored scale of a page that holds rows, brought up to a power of two (the
-// update calls store nothing else); 0 when it is no scale at all.
-__device__ __forceinline__ float pow2_up(float s) {
-  if (!(s >= 1.17549435e-38f && s <= 1.7014118e38f)) return 0.f;
-  const int bits = __float_as_int(s);
-  return (bits & 0x7fffff) ? __int_as_float((bits & 0x7f800000) + 0x00800000) : s;
+// The update calls store powers of two from 2^-24 to 2^9, under which x * (1 / scale) and
+// code * (old / new) are exact in fp32.
+__device__ __forceinline__ bool is_pow2_scale(float s) {
+  return (__float_as_int(s) & 0x7fffff) == 0 && s >= 5.9604645e-8f && s <= 512.f;
+}
+
+// x / scale rounded to the nearest whole number, ties to even, by its exact value; near: x / scale
+// to within 2^-22 of it. The remainder of the whole number next to `near` is exact (it is a
+// multiple of the last place of x or scale and at most about scale / 2), so that it shows
+// on which side of a tie the quotient lies.
+__device__ __forceinline__ float nearest(float x, float near, float scale) {
+  if (fabsf(x) >= 127.f * scale) return copysignf(127.f, x);
+  const float q = rintf(near), r = __fmaf_rn(-q, scale, x), half = 0.5f * scale;
+  const bool odd = static_cast<int>(q) & 1;
+  return fabsf(r) > half || (fabsf(r) == half && odd) ? q + copysignf(1.f, r) : q;
 }
 
 // Sequence of token t of a mixed pass: the first b with cu[b + 1] > t, or -1 when
@@ -209,11 +219,21 @@ __device__ __forceinline__ void write_rows(const Args& a, int64_t t, int b, int6
 
   float* sp = a.scales + page * 2 * a.hkv + which * a.hkv + h;
   int8_t* tile = (which ? a.v_cache : a.k_cache) + page * a.page_stride + h * a.head_stride;
-  const float stored = off > 0 ? *sp : 0.f;
-  const float scale = fmaxf(pow2_up(stored), __int_as_float((need_exp(amax) + 127) << 23));
+  float stored = off > 0 ? *sp : 0.f;
+  if (!(stored >= 0.f && stored <= 3.4028235e38f)) {  // no scale: the rows hold no values
+    raise_error(CIE_DEVERR_BAD_SCALE);
+    stored = 0.f;
+  }
+  const float scale = fmaxf(stored, __int_as_float((need_exp(amax) + 127) << 23));
   if (off > 0 && scale != stored) {
-    // the page's older rows (0 .. off - 1) under the new scale
-    const float ratio = pow2_up(stored) > 0.f ? __fdiv_rn(stored, scale) : 0.f;
+    // the page's older rows (0 .. off - 1) under the new scale, which is a power of two, so
+    // that the ratio is exact; the product is too when the old scale was one
+    const float ratio = __fdiv_rn(stored, scale);
+    const bool exact = is_pow2_scale(stored);
+    auto recode = [&](signed char c) {
+      return static_cast<signed char>(exact ? __float2int_rn(c * ratio)
+                                            : __double2int_rn(c * static_cast<double>(ratio)));
+    };
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int row = 4 * i + r;
@@ -222,24 +242,29 @@ __device__ __forceinline__ void write_rows(const Args& a, int64_t t, int b, int6
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           char4 v = d[k];
-          v.x = static_cast<signed char>(__float2int_rn(v.x * ratio));
-          v.y = static_cast<signed char>(__float2int_rn(v.y * ratio));
-          v.z = static_cast<signed char>(__float2int_rn(v.z * ratio));
-          v.w = static_cast<signed char>(__float2int_rn(v.w * ratio));
+          v.x = recode(v.x);
+          v.y = recode(v.y);
+          v.z = recode(v.z);
+          v.w = recode(v.w);
           d[k] = v;
         }
       }
     }
   }
-  const float inv = __fdiv_rn(1.f, scale);  // exact: scale is a power of two
+  const bool exact = is_pow2_scale(scale);
+  const float inv = __fdiv_rn(1.f, scale);
+  auto code = [&](float x) {
+    float q = __fmul_rn(x, inv);
+    if (!exact) q = nearest(x, q, scale);
+    return __float2int_rn(fminf(fmaxf(q, -127.f), 127.f));
+  };
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int row = 4 * i + r;
     if (row < n) {
       int q[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        q[e] = __float2int_rn(fminf(fmaxf(__fmul_rn(x[i][e], inv), -127.f), 127.f));
+      for (int e = 0; e < 8; ++e) q[e] = code(x[i][e]);
       uint2 u;
       u.x = (q[0] & 255) | (q[1] & 255) << 8 | (q[2] & 255) << 16 | q[3] << 24;
       u.y = (q[4] & 255) | (q[5] & 255) << 8 | (q[6] & 255) << 16 | q[7] << 24;
@@ -370,8 +395,9 @@ __device__ __forceinline__ __half2 two_codes(uint32_t w, uint32_t sel) {
   return __hsub2(*reinterpret_cast<const __half2*>(&h), __floats2half2_rn(1152.f, 1152.f));
 }
 
-// 8 codes -> 8 fp16 values code * scale, rounded once (exact for the powers of two that
-// the update calls store): in fp16 when the scale is a fp16 number, else in fp32.
+// 8 codes -> 8 fp16 values code * scale: rounded once, in fp16, when the scale is a fp16
+// number (exact for the powers of two that the update calls store), else rounded to fp32
+// and then to fp16.
 __device__ __forceinline__ uint4 dequant8(uint2 codes, float scale) {
   const uint32_t w[2] = {codes.x ^ 0x80808080u, codes.y ^ 0x80808080u};
   const __half s = __float2half_rn(scale);

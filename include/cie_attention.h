@@ -54,7 +54,8 @@ enum cie_device_error_bits {
   CIE_DEVERR_BAD_OFFSET = 1u << 3,    /* in-page offset outside [0, page_size)    */
   CIE_DEVERR_WAIT_TIMEOUT = 1u << 4,  /* an mbarrier wait ran past its limit      */
   CIE_DEVERR_BAD_SEQLENS = 1u << 5,   /* cu_seqlens not monotone / beyond T       */
-  CIE_DEVERR_NONFINITE = 1u << 6      /* inf or NaN written to an 8-bit page      */
+  CIE_DEVERR_NONFINITE = 1u << 6,     /* inf or NaN written to an 8-bit page      */
+  CIE_DEVERR_BAD_SCALE = 1u << 7      /* 8-bit page with a scale < 0, inf or NaN  */
 };
 
 /* ---- library-wide ---------------------------------------------------------- */

@@ -26,7 +26,10 @@
  * brought to the new scale (rounded to nearest even). Powers of two keep that
  * exact but for the bits shifted out: a value is off by at most one step of its
  * page's final scale however often the page grew, and by half a step when its
- * page was written at once. code * scale is exact in fp16. Rows a call does
+ * page was written at once; code * scale is exact in fp16. Pages that another program
+ * filled may have any scale >= 0: it stays while the new rows fit, and then holds for
+ * these too. A stored scale that is negative, infinite or NaN holds no values: the update
+ * makes the older rows 0 and sets CIE_DEVERR_BAD_SCALE. Rows a call does
  * not write, and their codes, stay as they were unless the scale grew.
  * Values beyond +-65024 saturate; an infinity is stored saturated and a NaN as
  * 0, and both set CIE_DEVERR_NONFINITE. Pages may be shared by slots that read
@@ -153,7 +156,8 @@ int cie_rope_kv_q8_mixed_update_bt32(const void* qkv, int64_t qkv_tok_stride, co
 
 /*
  * Positions [starts[b], lens[b]) of slot slot_ids[b], dequantised into a fp16
- * pool of the same page ids: out[page, h, row] = fp16(code * scale). Everything
+ * pool of the same page ids: out[page, h, row] = fp16(code * scale) (a scale that is no
+ * fp16 number: by way of fp32). Everything
  * else in the fp16 pool stays as it was, so a pass that attends to fp16 pages
  * (cie_mixed_attention) reads the result through the same block table. k_out /
  * v_out: (n_pages, num_kv_heads, page_size, head_dim) fp16 with their own page
@@ -183,9 +187,10 @@ int cie_kv_q8_read_bt32(const void* k_cache, const void* v_cache, const float* k
  * num_kv_heads 1, 2 or 4; num_q_heads / num_kv_heads 1 to 8. num_splits <= 0:
  * cie_decode_q8_default_splits; workspace: cie_decode_workspace_bytes(batch,
  * num_q_heads, head_dim, splits) bytes, 16-byte aligned (NULL when one split).
- * Any finite scales give softmax(q k^T / 8) v of k = code * scale, v = code *
- * scale; the products are taken with the codes (exact in fp16) and scaled in
- * fp32, probabilities are rounded to fp16 as cie_decode_attention rounds them.
+ * Any scales whose scores fit fp32 and whose values fit fp16 give softmax(q k^T / 8) v
+ * of k = code * scale, v = code * scale; the products are taken with the codes (exact in
+ * fp16) and scaled in fp32, probabilities are rounded to fp16 as cie_decode_attention
+ * rounds them.
  */
 int cie_decode_q8_default_splits(int batch, int device);
 
