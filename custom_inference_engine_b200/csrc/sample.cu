@@ -729,7 +729,8 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
       // with no more than u of the kept mass before it, 3 the last kept token when 2
       // comes out behind it
       Place z{};
-      for (int turn = k64 > 0 && k64 < p.vocab ? 0 : p32 < 1.f ? 1 : 2; turn < 4;) {
+      const bool filter_p = !(p32 >= 1.f);  // (a NaN keeps nothing but the first token)
+      for (int turn = k64 > 0 && k64 < p.vocab ? 0 : filter_p ? 1 : 2; turn < 4;) {
         Query query{turn == 0 || turn == 3, turn == 2, turn == 0 ? static_cast<int>(k64) : kept,
                     turn == 1 ? static_cast<double>(p32) * all : static_cast<double>(u32) * mass};
         z = s.last(query);
@@ -738,7 +739,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
           kept = z.tokens + 1;
           mass = z.mass + z.weight;
         }
-        turn = turn == 0 ? (p32 < 1.f ? 1 : 2) : turn == 1 ? 2 : turn == 2 && z.tokens >= kept ? 3 : 4;
+        turn = turn == 0 ? (filter_p ? 1 : 2) : turn == 1 ? 2 : turn == 2 && z.tokens >= kept ? 3 : 4;
       }
       key = z.key;
       rank = z.rank;

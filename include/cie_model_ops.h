@@ -90,7 +90,8 @@ int cie_lm_head_argmax(const void* hidden, int64_t hidden_stride, const void* we
  *   top_p[r]  the shortest prefix whose mass is >= top_p times the mass of the
  *             top_k prefix (>= 1: all),
  *   min_p[r]  the tokens with w >= min_p (the maximum's w is 1; <= 0: all) --
- * and never fewer than one; out[r] is the first token of the order at which the
+ * and never fewer than one, which a NaN top_p or min_p leaves; out[r] is the first
+ * token of the order at which the
  * cumulative mass exceeds uniform[r] * (mass of the kept tokens), uniform in
  * [0, 1) (a number outside gives the first or the last kept token). Weights
  * and masses are fp64. temperature[r] <= 0 or NaN gives the row's first

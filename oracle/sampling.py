@@ -19,7 +19,7 @@ def sample_row(logits, u, temperature, top_k=0, top_p=1.0, min_p=0.0) -> int:
     n = len(x)
     if 0 < top_k < n:
         n = int(top_k)
-    if top_p < 1:
+    if not top_p >= 1:
         cum = np.cumsum(w[:n])
         before = np.concatenate(([0.0], cum[:-1]))
         n = max(1, int((before < float(top_p) * cum[-1]).sum()))
