@@ -817,7 +817,9 @@ at::Tensor sample_rows(const at::Tensor& logits, const at::Tensor& uniform,
                        const std::optional<at::Tensor>& top_p,
                        const std::optional<at::Tensor>& min_p) {
   check_rows(logits, "logits");
-  const int64_t rows = logits.numel() / std::max<int64_t>(logits.size(-1), 1);
+  int64_t rows = 1;
+  for (int64_t d = 0; d + 1 < logits.dim(); ++d) rows *= logits.size(d);
+  TORCH_CHECK(rows == 0 || logits.size(-1) > 0, "logits hold an empty row: no token to give");
   auto per_row = [&](const at::Tensor& t, at::ScalarType type, const char* name) {
     TORCH_CHECK(t.scalar_type() == type && t.is_contiguous() && t.numel() == rows, name,
                 " must be a contiguous ", c10::toString(type), " tensor with one value per row");

@@ -1,10 +1,10 @@
-"""Sampling calls at the edges of their definition: a NaN top_p."""
+"""Sampling calls at the edges of their definition: a NaN top_p, and rows without tokens."""
 import math
 
 import pytest
 import torch
 
-from custom_inference_engine_b200 import native
+from custom_inference_engine_b200 import cabi, native
 from oracle.sampling import sample_row
 
 pytestmark = pytest.mark.gpu
@@ -33,3 +33,16 @@ def test_a_nan_top_p_keeps_the_first_token(ops, cuda_device, rows, vocab, with_k
                        float(p[i])) for i in range(rows)]
     assert got.tolist() == want
     assert want[0] == 5 and want[2:] == x[2:].float().argmax(-1).tolist()
+
+
+def test_rows_without_tokens_are_refused(ops, cuda_device):
+    """There is no token to give: no output is left unwritten."""
+    none = torch.zeros(0, device=cuda_device)
+    for shape in ((4, 0), (0,), (2, 3, 0)):
+        x = torch.zeros(shape, device=cuda_device).half()
+        with pytest.raises(RuntimeError, match="empty row"):
+            ops.sample_rows(x, none, none)
+    with pytest.raises(RuntimeError):
+        cabi.sample_rows(torch.zeros(4, 0, device=cuda_device).half(), none, none)
+    empty = torch.zeros(0, 10, device=cuda_device).half()
+    assert ops.sample_rows(empty, none, none).shape == (0,)
