@@ -132,6 +132,13 @@ class Sampling:
     top_p: float = 1.0
     min_p: float = 0.0
 
+    def check_scalar(self) -> None:
+        """Raises ValueError unless every parameter is one value."""
+        for name, x in vars(self).items():
+            if torch.as_tensor(x).dim() != 0:
+                raise ValueError(f"Sampling.{name} must be one value for all rows here: which row "
+                                 f"a request gets changes from step to step")
+
     def columns(self, rows: int, device):
         """The op's four per-row tensors."""
         def column(x, dtype):

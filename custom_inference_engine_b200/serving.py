@@ -77,6 +77,8 @@ class DecodeBuckets:
     def __init__(self, runner, max_batch: int, buckets=DECODE_BUCKETS, sampling=None):
         from .model_runner import DecodeGraph
 
+        if sampling is not None:
+            sampling.check_scalar()
         self.runner = runner
         self.sizes = [b for b in buckets if b < max_batch] + [max_batch]
         self.sizes = sorted(set(self.sizes))
@@ -198,7 +200,7 @@ def summarize(requests, trim: float = 0.05) -> dict:
 class RunnerEngine:
     """``serve``'s engine on a ``PagedRunner``: mixed passes and decode steps
     from CUDA graphs captured per token bucket and per batch bucket; greedy, or
-    sampled with a ``Sampling``."""
+    sampled with a ``Sampling`` (one value for all requests)."""
 
     def __init__(self, runner, n_slots: int, sampling=None):
         self.runner = runner
