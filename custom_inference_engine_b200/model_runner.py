@@ -427,6 +427,8 @@ class DecodeGraph:
     def step(self, uniform=None) -> torch.Tensor:
         """The next tokens; ``uniform``: the random numbers of a sampled step, drawn from
         the runner's generator when not given."""
+        if self.uniform is None and uniform is not None:
+            raise ValueError("a greedy step takes no random numbers")
         if self.uniform is not None:
             if uniform is None:
                 self.uniform.uniform_(generator=self.runner.generator)

@@ -1,4 +1,4 @@
-"""What the serving engine refuses of a Sampling, on the host."""
+"""What the serving engine and the decode step refuse of a Sampling, on the host."""
 import pytest
 import torch
 
@@ -20,3 +20,13 @@ def test_the_engine_takes_one_value_for_all_requests(kw):
 def test_one_value_is_no_list():
     MR.Sampling(0.7, 50, 0.9, 0.01).check_scalar()
     MR.Sampling(torch.tensor(0.7), torch.tensor(5)).check_scalar()
+
+
+def test_a_greedy_step_refuses_random_numbers():
+    d = MR.DecodeGraph.__new__(MR.DecodeGraph)
+    d.uniform = d.graph = None
+    d.slots, d.tokens = [], torch.zeros(2, dtype=torch.long)
+    d._step = lambda: None
+    assert torch.equal(d.step(), d.tokens)
+    with pytest.raises(ValueError, match="greedy"):
+        d.step(torch.rand(2))
