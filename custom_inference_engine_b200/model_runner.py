@@ -312,7 +312,8 @@ class PagedRunner:
         random numbers, drawn from the runner's generator when not given."""
         rows = logits.shape[0]
         if uniform is None:
-            uniform = torch.rand(rows, generator=self.generator, device=logits.device)
+            uniform = torch.rand(rows, generator=self.generator, dtype=torch.float32,
+                                 device=logits.device)
         return torch.ops.inference.sample_rows(logits, uniform,
                                                *sampling.columns(rows, logits.device))
 
@@ -383,7 +384,7 @@ class DecodeGraph:
         self.graph = None
         self.uniform = None
         if sampling is not None:
-            self.uniform = torch.zeros(B, device=dev)
+            self.uniform = torch.zeros(B, dtype=torch.float32, device=dev)
             self.columns = sampling.columns(B, dev)
         if capture:
             # the tokens this warm-up produces are discarded: undo its writes
