@@ -84,7 +84,7 @@ int cie_kv_q8_decode_update_bt32(void* k_cache, void* v_cache, float* kv_scales,
  * written) and they go to slot slot_ids[b] at positions kv_lens[b] onward. The
  * pass is given by sequence and not by (page, offset) per row because a page's
  * rows are quantised together. When a slot appears in more than one sequence
- * with rows, the last one's are written. batch <= 65535.
+ * with rows, the last one's are written.
  */
 int cie_kv_q8_mixed_update(void* k_cache, void* v_cache, float* kv_scales,
                            const int64_t* cu_seqlens, const int64_t* kv_lens,
@@ -161,7 +161,7 @@ int cie_rope_kv_q8_mixed_update_bt32(const void* qkv, int64_t qkv_tok_stride, co
  * else in the fp16 pool stays as it was, so a pass that attends to fp16 pages
  * (cie_mixed_attention) reads the result through the same block table. k_out /
  * v_out: (n_pages, num_kv_heads, page_size, head_dim) fp16 with their own page
- * and head strides (elements). starts may be NULL (all 0).
+ * and head strides (elements). starts may be NULL (all 0). batch <= 65535.
  */
 int cie_kv_q8_read(const void* k_cache, const void* v_cache, const float* kv_scales,
                    const int64_t* starts, const int64_t* lens, const int64_t* slot_ids,
@@ -184,7 +184,7 @@ int cie_kv_q8_read_bt32(const void* k_cache, const void* v_cache, const float* k
  * cie_decode_attention over the 8-bit pool: one query token per sequence, sequence
  * b sees rows [0, lens[b]) of slot slot_ids[b], lens[b] == 0 gives a zero row.
  * q / o (1, batch, num_q_heads, head_dim) fp16 contiguous, 16-byte aligned.
- * num_kv_heads 1, 2 or 4; num_q_heads / num_kv_heads 1 to 8. num_splits <= 0:
+ * num_kv_heads 1, 2 or 4; num_q_heads / num_kv_heads 1 to 8; batch <= 65535. num_splits <= 0:
  * cie_decode_q8_default_splits; workspace: cie_decode_workspace_bytes(batch,
  * num_q_heads, head_dim, splits) bytes, 16-byte aligned (NULL when one split).
  * Any scales whose scores fit fp32 and whose values fit fp16 give softmax(q k^T / 8) v
