@@ -121,8 +121,7 @@ __device__ __forceinline__ int seq_pages(const int64_t* lens, const int64_t* slo
   // before the query token, which is then written and attended to as well
   int64_t L = lens_per_slot ? __ldcg(lens + slot) + 1 : __ldcg(lens + b);
   if (L < 0) L = 0;
-  const int64_t np = (L + kPage - 1) / kPage;
-  return static_cast<int>(np > bt_stride ? bt_stride : np);
+  return static_cast<int>(L > bt_stride * kPage ? bt_stride : (L + kPage - 1) / kPage);
 }
 
 // Contiguous pages per split (the same partition in the split and merge kernels).

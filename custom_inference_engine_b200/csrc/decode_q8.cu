@@ -70,7 +70,7 @@ struct Params {
   const float* scales;      // (n_pages, 2, HKV)
   const int64_t* lens;      // (B,) keys; after an update of the call (n_slots,) without the new row
   const int64_t* slot_ids;  // (B,)
-  BlockTable table;         // (n_slots, bt_stride)
+  BlockTable table;         // n_slots rows, bt_stride apart
   __half* o;                // (B, H_q, D)
   float* ws_acc;            // (B, S, H_q, D)
   float* ws_ml;             // (B, S, H_q, 2)
@@ -78,6 +78,7 @@ struct Params {
   int group;                // query heads per kv head, 1..8
   int after_update;         // q and each row's last page are the preceding kernel's
   int64_t n_pages, n_slots, bt_stride;
+  int64_t row_pages;        // entries of a block-table row
   int64_t page_stride, head_stride;
 };
 
@@ -126,7 +127,7 @@ __device__ __forceinline__ uint32_t codes_to_half2(uint32_t w, uint32_t sel, uin
 }
 
 __device__ __forceinline__ int seq_pages(const Params& p, int b) {
-  return decode::seq_pages(p.lens, p.slot_ids, b, p.n_slots, p.bt_stride, p.after_update);
+  return decode::seq_pages(p.lens, p.slot_ids, b, p.n_slots, p.row_pages, p.after_update);
 }
 
 // kAfterUpdate: the preceding kernel is the same call's update, which writes q and, of
@@ -174,9 +175,9 @@ __global__ void __launch_bounds__(32 * kWarps, 2) decode_q8_split_kernel(const P
     L = load(p.lens + slot) + 1;
   }
   if (L < 0) L = 0;
-  if ((L + kPage - 1) / kPage > p.bt_stride) {
+  if (L > p.row_pages * kPage) {
     if (threadIdx.x == 0) raise_error(CIE_DEVERR_BAD_LENGTH);
-    L = p.bt_stride * kPage;
+    L = p.row_pages * kPage;
   }
   const int Li = static_cast<int>(L), n_seq_pages = (Li + kPage - 1) / kPage;
   const int pps = decode::split_pages(n_seq_pages, p.num_splits);
@@ -600,6 +601,7 @@ int prepare(Params& p, const void* q, const void* k, const void* v, const float*
   p.n_pages = n_pages;
   p.n_slots = n_slots;
   p.bt_stride = bt_stride;
+  p.row_pages = kvq8::row_pages(bt_stride, n_pages);
   p.page_stride = page_stride;
   p.head_stride = head_stride;
   return CIE_OK;

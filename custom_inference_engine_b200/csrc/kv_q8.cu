@@ -52,7 +52,14 @@ struct Args {
   int64_t tokens;
   int batch, hq, hkv;
   int64_t n_pages, n_slots, bt_stride;
+  int64_t row_pages;      // entries of a block-table row
 };
+
+// A block-table row holds at most the pool's pages: rows that lie further apart are rows of a
+// wider table, whose other columns are not this one's.
+__host__ __device__ inline int64_t row_pages(int64_t bt_stride, int64_t n_pages) {
+  return bt_stride < n_pages ? bt_stride : n_pages;
+}
 
 // Launched as a programmatic dependent of the preceding kernel: nothing is read or written
 // before that one is done, and the next such kernel may be scheduled meanwhile.
@@ -142,7 +149,7 @@ __device__ __forceinline__ int led_rows(const Args& a, const int64_t* cu, int64_
     pos = a.kv_lens[b] + t - cu[b];
     if (t != cu[b] && (pos & (kPage - 1)) != 0) return 0;
   }
-  if (pos < 0 || pos / kPage >= a.bt_stride) {
+  if (pos < 0 || pos / kPage >= a.row_pages) {
     raise_error(CIE_DEVERR_BAD_LENGTH);
     return 0;
   }
@@ -386,6 +393,7 @@ struct ReadArgs {
   int hkv;
   int64_t n_pages, n_slots, bt_stride;
   int64_t page_stride, head_stride, out_page, out_head;
+  int64_t row_pages;      // entries of a block-table row
 };
 
 // Two biased codes (code + 128) of `w`, picked by the selector, as fp16 numbers: 0x64 over a
@@ -431,9 +439,9 @@ __global__ void __launch_bounds__(256) read_kernel(const ReadArgs a) {
     if (blockIdx.x == 0 && threadIdx.x == 0) raise_error(CIE_DEVERR_BAD_SLOT);
     return;
   }
-  if (len > a.bt_stride * kPage) {
+  if (len > a.row_pages * kPage) {
     if (blockIdx.x == 0 && threadIdx.x == 0) raise_error(CIE_DEVERR_BAD_LENGTH);
-    len = a.bt_stride * kPage;
+    len = a.row_pages * kPage;
   }
   if (start < 0) start = 0;
   const int which = (threadIdx.x >> 5) & 1;
@@ -582,7 +590,7 @@ int read(const ReadArgs& a, int batch, int head_dim, int page_size, cie_stream_t
   // lengths are on the device: as many CTAs as the SMs hold, at most one per four pages of
   // the block-table row
   int64_t per = (8LL * sm_count() + batch - 1) / batch;
-  if (per > (a.bt_stride + 3) / 4) per = (a.bt_stride + 3) / 4;
+  if (per > (a.row_pages + 3) / 4) per = (a.row_pages + 3) / 4;
   return launch("kv_q8 read", read_kernel, dim3(static_cast<unsigned>(per), batch), stream, a);
 }
 
@@ -600,6 +608,7 @@ Args pool_args(void* k_cache, void* v_cache, float* scales, const int64_t* slot_
   a.n_pages = n_pages;
   a.n_slots = n_slots;
   a.bt_stride = bt_stride;
+  a.row_pages = row_pages(bt_stride, n_pages);
   a.page_stride = page_stride;
   a.head_stride = head_stride;
   return a;
@@ -710,7 +719,8 @@ int cie_kv_q8_read(const void* k_cache, const void* v_cache, const float* kv_sca
                               slot_ids, cie::BlockTable{block_table, 1},
                               static_cast<__half*>(k_out), static_cast<__half*>(v_out),
                               num_kv_heads, n_pages, n_slots, bt_stride, cache_page_stride,
-                              cache_head_stride, out_page_stride, out_head_stride};
+                              cache_head_stride, out_page_stride, out_head_stride,
+                              cie::kvq8::row_pages(bt_stride, n_pages)};
   return cie::kvq8::read(a, batch, head_dim, page_size, stream);
 }
 
@@ -793,7 +803,8 @@ int cie_kv_q8_read_bt32(const void* k_cache, const void* v_cache, const float* k
                               slot_ids, cie::BlockTable{block_table, 0},
                               static_cast<__half*>(k_out), static_cast<__half*>(v_out),
                               num_kv_heads, n_pages, n_slots, bt_stride, cache_page_stride,
-                              cache_head_stride, out_page_stride, out_head_stride};
+                              cache_head_stride, out_page_stride, out_head_stride,
+                              cie::kvq8::row_pages(bt_stride, n_pages)};
   return cie::kvq8::read(a, batch, head_dim, page_size, stream);
 }
 

@@ -15,6 +15,8 @@
  *               code * scale
  *   block_table, lens, slot_ids, cu_seqlens, kv_lens: as in cie_attention.h; the
  *               *_bt32 variants take the table as int32 page ids
+ *               (a row holds min(bt_stride, n_pages) pages: longer lengths set
+ *               CIE_DEVERR_BAD_LENGTH, also where rows of a wider table lie further apart)
  * head_dim 64, page_size 16.
  *
  * What the update calls store: the scale of (page, K or V, kv head) is
