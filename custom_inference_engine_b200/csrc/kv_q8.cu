@@ -236,42 +236,48 @@ __device__ __forceinline__ void write_rows(const Args& a, int64_t t, int b, int6
     // the page's older rows (0 .. off - 1) under the new scale, which is a power of two, so
     // that the ratio is exact; the product is too when the old scale was one
     const float ratio = __fdiv_rn(stored, scale);
-    const bool exact = is_pow2_scale(stored);
-    auto recode = [&](signed char c) {
-      return static_cast<signed char>(exact ? __float2int_rn(c * ratio)
-                                            : __double2int_rn(c * static_cast<double>(ratio)));
-    };
+    auto recode_all = [&](auto recode) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = 4 * i + r;
-      if (row < off) {
-        char4* d = reinterpret_cast<char4*>(tile + row * kD + 8 * c);
+      for (int i = 0; i < 4; ++i) {
+        const int row = 4 * i + r;
+        if (row < off) {
+          char4* d = reinterpret_cast<char4*>(tile + row * kD + 8 * c);
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          char4 v = d[k];
-          v.x = recode(v.x);
-          v.y = recode(v.y);
-          v.z = recode(v.z);
-          v.w = recode(v.w);
-          d[k] = v;
+          for (int k = 0; k < 2; ++k) {
+            char4 v = d[k];
+            v.x = static_cast<signed char>(recode(v.x));
+            v.y = static_cast<signed char>(recode(v.y));
+            v.z = static_cast<signed char>(recode(v.z));
+            v.w = static_cast<signed char>(recode(v.w));
+            d[k] = v;
+          }
         }
       }
+    };
+    if (is_pow2_scale(stored)) {
+      recode_all([&](signed char q) { return __float2int_rn(q * ratio); });
+    } else {
+      recode_all([&](signed char q) { return __double2int_rn(q * static_cast<double>(ratio)); });
     }
   }
-  const bool exact = is_pow2_scale(scale);
-  const float inv = __fdiv_rn(1.f, scale);
-  auto code = [&](float x) {
-    float q = __fmul_rn(x, inv);
-    if (!exact) q = nearest(x, q, scale);
-    return __float2int_rn(fminf(fmaxf(q, -127.f), 127.f));
-  };
+  float inv = __fdiv_rn(1.f, scale);
+  if (!is_pow2_scale(scale)) {  // (outside the loop below: one branch instead of 32)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (4 * i + r < n) x[i][e] = nearest(x[i][e], __fmul_rn(x[i][e], inv), scale);
+    }
+    inv = 1.f;
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int row = 4 * i + r;
     if (row < n) {
       int q[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) q[e] = code(x[i][e]);
+      for (int e = 0; e < 8; ++e)
+        q[e] = __float2int_rn(fminf(fmaxf(__fmul_rn(x[i][e], inv), -127.f), 127.f));
       uint2 u;
       u.x = (q[0] & 255) | (q[1] & 255) << 8 | (q[2] & 255) << 16 | q[3] << 24;
       u.y = (q[4] & 255) | (q[5] & 255) << 8 | (q[6] & 255) << 16 | q[7] << 24;
