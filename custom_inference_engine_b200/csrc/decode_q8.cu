@@ -8,7 +8,10 @@
 // Codes are whole numbers up to 127, exact in fp16: a byte c + 128 under the
 // exponent byte 0x64 is the fp16 number 1024 + 128 + c, and subtracting 1152 is
 // exact. scale_k and scale_v multiply fp32 results, so neither p nor a code is
-// ever scaled in fp16, whatever range the page scales span.
+// ever scaled in fp16, whatever range the page scales span. p has the 11 bits of the MMA's
+// operand: a second MMA on its remainder would double the P V products for an error that is
+// the output's own rounding already (against 64 bits, as a share of the norm: 2.2e-4 to 2.4e-4,
+// with 32-bit probabilities 2.0e-4 to 2.3e-4). Its sum l is of the fp32 values.
 //
 // Contraction indices and output rows may be numbered freely as long as both
 // operands agree, so every lane's operand bytes are contiguous in memory and the two
@@ -32,9 +35,11 @@
 // The warps' results are merged in shared memory, those of several splits by a second
 // kernel.
 //
-// Measured (B200, cold pages): 256 x 4096 rows, two heads, 51 us = 5.3 TB/s, 0.81 of the
-// measured copy bandwidth; 64 x 16001-32768 80 us; one sequence of 511 rows 4.5 us, of
-// 16384 7.8 us. What bounds it: the pages' bandwidth at large sizes, with 16 warps per SM
+// Measured (B200, cold pages, a chain of calls in a graph, where a call's start overlaps the
+// one before): 256 x 4096 rows, two heads, 52 us = 5.2 TB/s, 0.80 of the measured copy
+// bandwidth; 64 x 16001-32768 83 us; one sequence of 511 rows 4.5 us, of 16384 7.4 us. Calls
+// between events take 4 to 5 us more (56, 87 and 9.7 us for the first three). What bounds it:
+// the pages' bandwidth at large sizes, with 16 warps per SM
 // (128 registers) and about 240 instructions a page and head; the chain slot -> length ->
 // block table -> page -> merge at small ones.
 #include "cie_common.cuh"
@@ -133,7 +138,8 @@ __device__ __forceinline__ int seq_pages(const Params& p, int b) {
 // kAfterUpdate: the preceding kernel is the same call's update, which writes q and, of
 // every row's pages, the last one, with its scale. It has itself waited for everything before
 // it when this grid starts, so that a warp's first pages are fetched while it runs (64 rows
-// of 650 keys: 12.7 us for the call, 15.1 us as two calls; 256 of 2000: 42.2 and 46.3).
+// of 325 to 975 keys: 12.9 us for the call, 14.0 us as two calls; 256 of 1000 to 3000: 42.1 and
+// 45.8). With two heads it spills 4 bytes at the cap of 128 registers.
 // Rotating q here as well and waiting only before the last page is read won 0.7 to 1.5 us at
 // 64 rows and lost 1.4 to 2.2 us at 256 (registers let one CTA of two start beside the update).
 template <int HKV, bool kAfterUpdate>
@@ -677,11 +683,14 @@ int cie_decode_q8_default_splits(int batch, int device) {
       sms = n;
   }
   if (batch <= 0) return 1;
-  // Two CTAs per SM, as the smallest power of two that is at least 4/5 of that. More CTAs
-  // even out ragged batches, where the longest split sets the time (256 sequences of 1 to
-  // 4096 rows, one kv head: 29.1 us at 1 split, 21.7 at 2, 25.7 at 4; 100 of 1 to 4000,
-  // four heads: 39.0 at 2, 26.4 at 4), but cost even ones a second wave and a merge
-  // (256 x 4096, two heads: 49.8 us at 1 split, 55.2 at 2; 64 x 4096: 18.6 at 4, 20.4 at 8).
+  // Two CTAs per SM, as the smallest power of two that is at least 4/5 of that, and 64 at
+  // most. More CTAs even out ragged batches, where the longest split sets the time (256
+  // sequences of 1 to 4096 rows, one kv head: 32 us at 1 split, 29 at 2, 31 at 4; 100 of 1 to
+  // 4000, four heads: 50 at 2, 38 at 4), but cost even ones a second wave and a merge
+  // (256 x 4096, two heads: 53 us at 1 split, 58 at 2; 64 x 4096: 20 at 4, 24 at 8). The cap
+  // leaves one or two sequences 64 or 128 CTAs of the 296 places: right up to 16384 rows (one:
+  // 7.4 us at 64, 7.9 at 128; two: 7.6 and 9.2) and about even at 32768 (9.2 and 8.7; 10.2 and
+  // 11.4); one of 131072 rows would take 15.6 us at 128 instead of 21.7, two 20.9 instead of 22.2.
   int s = 1;
   while (s < 64 && 5LL * s * batch < 8LL * sms) s *= 2;
   return s;

@@ -294,7 +294,7 @@ __device__ __forceinline__ void write_rows(const Args& a, int64_t t, int b, int6
 // the chain of dependent loads (cu_seqlens -> length, slot -> block table -> scale), so
 // a CTA gets few units and the two kinds of work run side by side.
 // Measured (B200, device time, q rotated too): a decode step of 8 rows 4.0 us, of 256 5.3 us, a
-// mixed pass of 2048 rows 6.2 us (with the read back 9.8 us; 21.9 us with one kind of CTA).
+// mixed pass of 2048 rows 6.2 us (with the read back 10.0 us; 21.9 us with one kind of CTA).
 constexpr int kTile = 4;
 constexpr int kCuShared = 512;  // cu_seqlens entries that are searched in shared memory
 
@@ -436,6 +436,8 @@ __device__ __forceinline__ uint4 dequant8(uint2 codes, float scale) {
 // 512-byte writes), two heads' reads in flight before their first write; a sequence's
 // pages are dealt to its warps one by one. Bound by bandwidth, 1 byte read and 2 written
 // a value: 32 x 8191 rows 19.0 us = 5.3 TB/s on a B200, 0.81 of a copy; 2047 rows 2.3 us.
+// CTAs are dealt per sequence, absent ones too, so that one long history among them has few:
+// 8191 rows alone 2.7 us, among 31 empty sequences 5.8 us, 63 8.9 us, 255 27 us.
 __global__ void __launch_bounds__(256) read_kernel(const ReadArgs a) {
   const int b = blockIdx.y, lane = threadIdx.x & 31;
   start_as_dependent();

@@ -31,8 +31,11 @@
 // 256 rows of 32003 27 us; with top-k, top-p and min-p 2 to 4 us more. What bounds it, of the 16 us of a CTA
 // that counts 75968 tokens: shared atomics on random banks 6.5 us (6 tokens a cycle), the
 // chunks' sums 4 us (fp64 latency, and distributed shared memory at about 22 bytes a cycle
-// and SM), each search 1.7 us (one warp), clearing, barriers and look-up the rest. 128 KiB of
-// counters allow one CTA per SM, so that more than 148 of them take another wave.
+// and SM), each search 1.7 us (one warp), clearing, barriers and look-up the rest. One CTA
+// runs per SM, for two reasons: 126 to 128 registers x 512 threads are all that an SM has, and
+// 181 KiB of shared memory (128 of them counters, 53 the searches' tables) more than half. So
+// more than 148 CTAs take another wave: 256 rows of 151936, in clusters of two, 87 us.
+// The clusters of eight spill 68 bytes.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
