@@ -10,8 +10,8 @@
 // exact. scale_k and scale_v multiply fp32 results, so neither p nor a code is
 // ever scaled in fp16, whatever range the page scales span. p has the 11 bits of the MMA's
 // operand: a second MMA on its remainder would double the P V products for an error that is
-// the output's own rounding already (against 64 bits, as a share of the norm: 2.2e-4 to 2.4e-4,
-// with 32-bit probabilities 2.0e-4 to 2.3e-4). Its sum l is of the fp32 values.
+// the output's own rounding already (against 64 bits, as a share of the norm: 2.2e-4 to 2.5e-4,
+// with 32-bit probabilities 1.9e-4 to 2.3e-4). Its sum l is of the fp32 values.
 //
 // Contraction indices and output rows may be numbered freely as long as both
 // operands agree, so every lane's operand bytes are contiguous in memory and the two
